@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * N16_WAVES, N16_WPE(KBN, RT)) void mmd_n16_kern
         }
         PHASE_MARK(2);
 
-        // 2. E = expm1(-t), two values per instruction (v_pk_*_f32); h = 0: points 4 g, 4 g + 1; h = 1: + 2, + 3.
+        // 2. E = expm1(-t), two values at a time; h = 0: points 4 g, 4 g + 1; h = 1: + 2, + 3.
         // One row tile at a time, through to its E pieces in LDS (short live ranges: the register budget of two or
         // three waves per SIMD is what this kernel lives on).
         const f32x4 cn = *reinterpret_cast<const f32x4*>(sm + L::NORM_OFF + buf * 256 + u * 64 + 16 * g);
