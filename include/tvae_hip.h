@@ -46,6 +46,9 @@ extern "C" {
  * three-product form when the points' norms are large against latent_size. */
 #define TVAE_F32_STRICT 2
 
+/* tvae_dropout and tvae_norm_* only. */
+#define TVAE_F16 3
+
 #define TVAE_OK 0
 #define TVAE_ERR_ARG 1         /* bad shape / null pointer / unsupported size */
 #define TVAE_ERR_HIP 2         /* a HIP runtime call failed */
@@ -284,6 +287,54 @@ int tvae_rbf_kernel_bwd(const float* x, const float* y, const float* K, const fl
  * immediately before / after the dominant kernel (mmd_tile_kernel), so bench.py can time that
  * kernel live with HIP events.  One-shot; pass NULLs to disarm.  Events are hipEvent_t as void*. */
 int tvae_profile_next_mmd(void* ev_start, void* ev_stop);
+
+/* ---------------------------------------------------------------------------------
+ * Dropout, alone or added to a residual, with a mask that is never stored:
+ *     out(i, c) = [residual(i, c) +] (kept(i, c) ? in(i, c) * scale : 0)
+ * kept(i, c) depends on (seed, offset, i, c) alone: Philox4x32 with ten rounds, key = seed,
+ * counter = (c / 8, i, offset low 32 bits, offset high); its four words are eight 16-bit draws for
+ * the columns 8 (c / 8) .. + 7, low half first, and an element is dropped where its draw is below
+ * T = round(65536 p) (half to even).  scale = 65536 / (65536 - T).  p = 0 copies, p = 1 gives zeros.
+ * The backward pass is the same call on the cotangent, without a residual.
+ *   in       rows of d elements: element (i, c) at (i / grp) * in_so + (i % grp) * in_si + c
+ *            (dense: grp 1, in_so d; the first n tokens of a (B, S, d) tensor: grp n, in_so S d, in_si d)
+ *   residual nullable, of out's type, rows laid out by (grp, res_so, res_si)
+ *   out      (rows, d) dense; may not overlap the inputs
+ *   rng      DEVICE pointer to {seed, offset} as two 64-bit words, read when the kernel runs (a replayed
+ *            graph sees new ones); NULL: `seed` and `offset` of the call
+ *   types    TVAE_F32, TVAE_BF16 or TVAE_F16; in and out of one type, or one of them fp32
+ * ------------------------------------------------------------------------------- */
+int tvae_dropout(const void* in, int64_t in_so, int64_t in_si, const void* residual, int64_t res_so, int64_t res_si,
+                 int64_t grp, void* out, int64_t rows, int64_t d, double p, const int64_t* rng, uint64_t seed,
+                 uint64_t offset, int in_dtype, int out_dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Layer norm and RMS norm over rows of d, with the residual sum and dropout that stand before them:
+ *     v = [residual +] dropout(x)          (as tvae_dropout; x or residual may be NULL, not both)
+ *     TVAE_NORM_LAYER: y = (v - mean v) * rstd * weight + bias,  rstd = (mean (v - mean v)^2 + eps)^-1/2
+ *     TVAE_NORM_RMS:   y = v * rstd * weight,                    rstd = (mean v^2 + eps)^-1/2
+ * v stays fp32 between the loads and the stores.
+ *   x, y     `dtype` (TVAE_F32, TVAE_BF16, TVAE_F16); y (rows, d) dense
+ *   weight, bias  (d) of `w_dtype`: `dtype` or TVAE_F32; NULL: 1 and 0 (RMS norm: bias NULL)
+ *   residual, sum `r_dtype`: `dtype` or TVAE_F32; sum (rows, d) dense receives v, nullable
+ *   mean, rstd    (rows) fp32 for the backward pass; NULL in inference (RMS norm: mean NULL) */
+#define TVAE_NORM_LAYER 0
+#define TVAE_NORM_RMS 1
+int tvae_norm_fwd(int kind, const void* x, int64_t x_so, int64_t x_si, const void* residual, int64_t res_so, int64_t res_si,
+                  int64_t grp, const void* weight, const void* bias, double eps, double p, const int64_t* rng, uint64_t seed,
+                  uint64_t offset, void* y, void* sum, float* mean, float* rstd, int64_t rows, int64_t d, int dtype,
+                  int w_dtype, int r_dtype, void* stream);
+
+/* Backward.  dy (rows, d) `dtype` with its own row strides; dsum (r_dtype, nullable) the cotangent of `sum`.
+ * v is formed again from x and residual as in the forward call; a caller that kept an fp32 `sum` passes it as
+ * `residual` with x NULL and the same p and rng (they still shape dx).  Outputs, all nullable and dense:
+ * dx (`dtype`), dresidual (`r_dtype`), dweight and dbias (`w_dtype`).  The sums over rows have a fixed order. */
+int64_t tvae_norm_bwd_workspace_bytes(int64_t rows, int64_t d);
+int tvae_norm_bwd(int kind, const void* dy, int64_t dy_so, int64_t dy_si, const void* dsum, int64_t ds_so, int64_t ds_si,
+                  const void* x, int64_t x_so, int64_t x_si, const void* residual, int64_t res_so, int64_t res_si, int64_t grp,
+                  const void* weight, const float* mean, const float* rstd, double p, const int64_t* rng, uint64_t seed,
+                  uint64_t offset, void* dx, void* dresidual, void* dweight, void* dbias, int64_t rows, int64_t d, int dtype,
+                  int w_dtype, int r_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

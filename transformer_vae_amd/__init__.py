@@ -8,6 +8,7 @@ from .autoencoders import (EncoderDecoderVAE, LatentDecoder, LatentDecoderFunnel
                            LatentDecoderT5Norm, LatentEncoderLargeTanh, LatentEncoderNTokens, VAE_DECODER_MODELS,
                            VAE_ENCODER_MODELS)
 from .model_outputs import BaseVAE_Output
+from .norms import Dropout, DropoutAddLayerNorm, DropoutAddRMSNorm, LayerNorm, RMSNorm
 from .utils import slerp, upsample
 from . import losses, trainer
 from .graph import GraphedStep
@@ -16,4 +17,5 @@ build = _lib.build
 
 __all__ = ["EncoderDecoderVAE", "LatentEncoderNTokens", "LatentEncoderLargeTanh", "LatentDecoderNTokens",
            "LatentDecoderFunnelNorm", "LatentDecoderT5Norm", "LatentDecoder", "VAE_ENCODER_MODELS",
-           "VAE_DECODER_MODELS", "BaseVAE_Output", "slerp", "upsample", "losses", "trainer", "GraphedStep", "build"]
+           "VAE_DECODER_MODELS", "BaseVAE_Output", "slerp", "upsample", "losses", "trainer", "GraphedStep", "LayerNorm",
+           "RMSNorm", "Dropout", "DropoutAddLayerNorm", "DropoutAddRMSNorm", "build"]

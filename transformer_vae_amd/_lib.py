@@ -18,8 +18,11 @@ LIB_PATH = os.path.join(_HERE, "libtvae_hip.so")
 HEADER = os.path.join(os.path.dirname(_HERE), "include", "tvae_hip.h")
 
 TVAE_F32, TVAE_BF16, TVAE_F32_STRICT = 0, 1, 2      # TVAE_F32_STRICT: tvae_mmd_* only (include/tvae_hip.h)
+TVAE_F16 = 3                                        # tvae_dropout and tvae_norm_* only
+TVAE_NORM_LAYER, TVAE_NORM_RMS = 0, 1
 
 _i64, _vp, _int, _f32, _f64 = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_double
+_u64 = ctypes.c_uint64
 
 # name -> (restype, argtypes); mirrors include/tvae_hip.h one to one
 SIGNATURES = {
@@ -64,6 +67,17 @@ SIGNATURES = {
     # dgamma, dbeta, B, S, n_eff, d, L, dtype, workspace, bytes, stream
     "tvae_small_step_bwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
                                    _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _i64, _vp]),
+    # in, so, si, residual, so, si, grp, out, rows, d, p, rng, seed, offset, in_dtype, out_dtype, stream
+    "tvae_dropout": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _f64, _vp, _u64, _u64, _int, _int, _vp]),
+    # kind, x, so, si, residual, so, si, grp, weight, bias, eps, p, rng, seed, offset, y, sum, mean, rstd, rows, d, dtype,
+    # w_dtype, r_dtype, stream
+    "tvae_norm_fwd": (_int, [_int, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _f64, _f64, _vp, _u64, _u64, _vp, _vp, _vp,
+                             _vp, _i64, _i64, _int, _int, _int, _vp]),
+    "tvae_norm_bwd_workspace_bytes": (_i64, [_i64] * 2),
+    # kind, dy, so, si, dsum, so, si, x, so, si, residual, so, si, grp, weight, mean, rstd, p, rng, seed, offset, dx, dresidual,
+    # dweight, dbias, rows, d, dtype, w_dtype, r_dtype, workspace, bytes, stream
+    "tvae_norm_bwd": (_int, [_int, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _f64,
+                             _vp, _u64, _u64, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _int, _vp, _i64, _vp]),
 }
 
 _lock = threading.Lock()

@@ -15,7 +15,9 @@ Additions that default to the reference's behaviour:
   * ``true_samples=`` on ``EncoderDecoderVAE.forward`` injects the prior sample (the
     reference draws ``torch.randn(latent.size())`` inside ``_regularliser_loss``, :135);
   * ``mmd_scope="global"`` + ``process_group`` evaluate the MMD of the global batch,
-    row-sharded over ranks (distributed.py); ``"local"`` is what the reference does under DDP.
+    row-sharded over ranks (distributed.py); ``"local"`` is what the reference does under DDP;
+  * ``dropout_rate`` of the decoders (or ``config.latent_decoder_dropout``): dropout on the decoded tokens in training, where
+    a sub-layer of their kind has it -- before the norm of the default decoder, on the branch of ``t5_norm``.
 """
 from __future__ import annotations
 
@@ -52,8 +54,13 @@ class LatentDecoderNTokens(nn.Module):
 
     When latent_size == d_model the reference installs an identity (and no parameters); so do we."""
 
-    def __init__(self, config):
+    dropout_rate = 0.0
+
+    def __init__(self, config, dropout_rate=None):
         super().__init__()
+        self.dropout_rate = float(getattr(config, "latent_decoder_dropout", 0.0) if dropout_rate is None else dropout_rate)
+        if not 0.0 <= self.dropout_rate <= 1.0:
+            raise ValueError(f"dropout_rate must be between 0 and 1, got {self.dropout_rate}")
         self.latent_size = config.latent_size
         if self.latent_size == config.t5.d_model:
             logger.warning("Latent decoder is not rescaling the latent code.")
@@ -66,33 +73,48 @@ class LatentDecoderNTokens(nn.Module):
             return None, None
         return self.latent_to_token.weight, self.latent_to_token.bias
 
-    def forward(self, latent) -> torch.Tensor:
+    def _active_dropout(self) -> float:
+        return self.dropout_rate if self.training else 0.0
+
+    def _decode(self, latent) -> torch.Tensor:
         w, b = self._linear_params()
         if w is None:
             return latent          # identity, exactly like the reference's `lambda x: x`
         return F.latent_decode(latent, w, b)
 
+    def forward(self, latent) -> torch.Tensor:
+        out, p = self._decode(latent), self._active_dropout()
+        return F.dropout(out, p) if p > 0.0 else out
+
 
 class LatentDecoderFunnelNorm(LatentDecoderNTokens):
     """Linear + nn.LayerNorm(funnel.d_model, funnel.layer_norm_eps), fused (autoencoders.py:58-67)."""
 
-    def __init__(self, config):
-        super().__init__(config)
+    def __init__(self, config, dropout_rate=None):
+        super().__init__(config, dropout_rate)
         self.norm = nn.LayerNorm(config.funnel.d_model, config.funnel.layer_norm_eps)
 
     def forward(self, latent) -> torch.Tensor:
         w, b = self._linear_params()
+        p = self._active_dropout()
+        if p > 0.0:                # LayerNorm(dropout(linear)), as the Funnel's own sub-layers order them
+            r = self._decode(latent)
+            g, c = (t if t.dtype in (r.dtype, torch.float32) else t.float() for t in (self.norm.weight, self.norm.bias))
+            return F.dropout_add_layer_norm(r, None, g, c, self.norm.eps, p)
         return F.latent_decode(latent, w, b, self.norm.weight, self.norm.bias, self.norm.eps)
 
 
 class LatentDecoderT5Norm(LatentDecoderNTokens):
     """Linear + a stock HF ``T5LayerFF`` block with dropout forced to 0 (autoencoders.py:42-55).
 
-    The feed-forward block is third-party code in the reference too; only the linear runs on
-    our kernels."""
+    The feed-forward block is third-party code in the reference too; by default only the linear runs on
+    our kernels.  ``native_norm`` (or ``config.latent_decoder_native_norm``; always with a dropout rate): the block's
+    norm, dropout and residual sum run on our kernels too, its two products stay where they are; same parameters."""
 
-    def __init__(self, config):
-        super().__init__(config)
+    def __init__(self, config, dropout_rate=None, native_norm=None):
+        super().__init__(config, dropout_rate)
+        native = getattr(config, "latent_decoder_native_norm", False) if native_norm is None else native_norm
+        self.native_norm = bool(native) or self.dropout_rate > 0.0
         from transformers.models.t5.modeling_t5 import T5LayerFF
         t_config = config.t5
         dropout_rate = t_config.dropout_rate
@@ -101,7 +123,13 @@ class LatentDecoderT5Norm(LatentDecoderNTokens):
         t_config.dropout_rate = dropout_rate
 
     def forward(self, latent) -> torch.Tensor:
-        return self.norm(super().forward(latent))
+        h = self._decode(latent)
+        if not self.native_norm:
+            return self.norm(h)
+        ln = self.norm.layer_norm
+        weight = ln.weight if ln.weight.dtype in (h.dtype, torch.float32) else ln.weight.float()
+        branch = self.norm.DenseReluDense(F.rms_norm(h, weight, ln.variance_epsilon))
+        return F.dropout_add(branch, h if h.dtype == branch.dtype else h.float(), self._active_dropout())
 
 
 # alias for the name used in the north-star description
@@ -165,6 +193,8 @@ class EncoderDecoderVAE(nn.Module):
         if not h.is_cuda or h.dim() != 3 or h.dtype not in (torch.float32, torch.bfloat16):
             return False
         if h.shape[0] * min(int(enc.n_tokens), h.shape[1]) == 0 or h.shape[2] != enc.token_to_latent.weight.shape[1]:
+            return False
+        if dec._active_dropout() > 0.0:
             return False
         if dec.latent_to_token is None and not isinstance(dec, LatentDecoderFunnelNorm):
             return False                      # identity decoder: reconstructed_encoding IS the latent tensor
