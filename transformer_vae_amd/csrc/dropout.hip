@@ -34,15 +34,15 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutCall c) {
         const long long row = t / c.groups;
         const int g = (int)(t - row * c.groups), col = 8 * g, nv = c.d - col;
         float v[8];
-        load8(static_cast<const A*>(c.in) + row_offset(c.in_rows, c.grp, row) + col, nv, v);
+        load8(static_cast<const A*>(c.in) + row_offset(c.in_rows, c.grp, row), col, nv, v);
         if (c.drop.threshold) drop8(ph, c.drop, (uint32_t)g, (uint32_t)row, v);
         if (c.residual) {
             float r[8];
-            load8(static_cast<const O*>(c.residual) + row_offset(c.res_rows, c.grp, row) + col, nv, r);
+            load8(static_cast<const O*>(c.residual) + row_offset(c.res_rows, c.grp, row), col, nv, r);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += r[e];
         }
-        store8(static_cast<O*>(c.out) + row * c.d + col, nv, v);
+        store8(static_cast<O*>(c.out) + row * c.d, col, nv, v);
     }
 }
 

@@ -6,56 +6,71 @@ namespace tvae {
 
 typedef _Float16 f16;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-// rows start wherever their stride puts them, so the 16-byte accesses below promise the element's own alignment only
-typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+// rows start wherever their stride puts them: the 16-byte accesses below promise the alignment of a 16-bit element only
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 
-// ---- eight neighbouring elements <-> fp32 ----------------------------------------------------------------------------
-__device__ __forceinline__ void load8_full(const float* p, float v[8]) {
-    const u32x4 a = *reinterpret_cast<const u32x4_a4*>(p), b = *reinterpret_cast<const u32x4_a4*>(p + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] = __uint_as_float(a[e]); v[4 + e] = __uint_as_float(b[e]); }
+// ---- elements <-> fp32 ----------------------------------------------------------------------------------------------------
+// NT: past the caches, for streams too long to be found there again
+template <bool NT>
+__device__ __forceinline__ u32x4 load16(const u32x4_a2* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(p);
+    else return *p;
 }
-__device__ __forceinline__ void load8_full(const bf16* p, float v[8]) {
-    const u32x4 a = *reinterpret_cast<const u32x4_a2*>(p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(a[e] << 16); v[2 * e + 1] = __uint_as_float(a[e] & 0xffff0000u); }
+template <bool NT>
+__device__ __forceinline__ void put16(u32x4_a2* p, u32x4 v) {
+    if constexpr (NT) __builtin_nontemporal_store(v, p);
+    else *p = v;
 }
-__device__ __forceinline__ void load8_full(const f16* p, float v[8]) {
-    const u32x4 a = *reinterpret_cast<const u32x4_a2*>(p);
+// eight elements in their type's own bits, which is what a load in flight keeps in registers
+template <typename T> struct Raw8 { u32x4 q[sizeof(T) / 2]; };
+
+// the first nv of four (fp32) or eight (16 bits) elements at p in 16 bytes; the others are 0
+template <bool NT>
+__device__ __forceinline__ u32x4 load_raw(const float* p, int nv) {
+    if (nv >= 4) return load16<NT>(reinterpret_cast<const u32x4_a2*>(p));
+    u32x4 q = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < nv) q[e] = reinterpret_cast<const uint32_t*>(p)[e];
+    return q;
+}
+template <bool NT, typename T>
+__device__ __forceinline__ u32x4 load_raw(const T* p, int nv) {
+    if (nv >= 8) return load16<NT>(reinterpret_cast<const u32x4_a2*>(p));
+    u32x4 q = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+        if (e < nv) q[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+    return q;
+}
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, float v[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r.q[e >> 2][e & 3]);
+}
+__device__ __forceinline__ void unpack8(const Raw8<bf16>& r, float v[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[2 * e] = __uint_as_float(r.q[0][e] << 16); v[2 * e + 1] = __uint_as_float(r.q[0][e] & 0xffff0000u); }
+}
+__device__ __forceinline__ void unpack8(const Raw8<f16>& r, float v[8]) {
     typedef f16 f16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const uint32_t w = a[e];        // a copy: the builtin takes a vector element for the vector's first
+        const uint32_t w = r.q[0][e];       // a copy: the builtin takes a vector element for the vector's first
         const f16x2 h = __builtin_bit_cast(f16x2, w);
         v[2 * e] = (float)h[0]; v[2 * e + 1] = (float)h[1];
     }
 }
-// the first nv (1..8) of eight; the others read as 0
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int nv, float v[8]) {
-    if (nv >= 8) {
-        load8_full(p, v);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < nv ? to_f32(p[e]) : 0.f;
-    }
+__device__ __forceinline__ u32x4 pack4(const float v[4]) {
+    return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
 }
-__device__ __forceinline__ void store8_full(float* p, const float v[8]) {
-    u32x4 a, b;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { a[e] = __float_as_uint(v[e]); b[e] = __float_as_uint(v[4 + e]); }
-    *reinterpret_cast<u32x4_a4*>(p) = a;
-    *reinterpret_cast<u32x4_a4*>(p + 4) = b;
-}
-__device__ __forceinline__ void store8_full(bf16* p, const float v[8]) {
+__device__ __forceinline__ u32x4 pack8(const float v[8], bf16) {
     u32x4 a;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         a[e] = (uint32_t)__bfloat16_as_ushort(__float2bfloat16(v[2 * e])) | ((uint32_t)__bfloat16_as_ushort(__float2bfloat16(v[2 * e + 1])) << 16);
-    *reinterpret_cast<u32x4_a2*>(p) = a;
+    return a;
 }
-__device__ __forceinline__ void store8_full(f16* p, const float v[8]) {
+__device__ __forceinline__ u32x4 pack8(const float v[8], f16) {
     typedef f16 f16x2 __attribute__((ext_vector_type(2)));
     u32x4 a;
 #pragma unroll
@@ -63,17 +78,60 @@ __device__ __forceinline__ void store8_full(f16* p, const float v[8]) {
         const f16x2 h = {(f16)v[2 * e], (f16)v[2 * e + 1]};
         a[e] = __builtin_bit_cast(uint32_t, h);
     }
-    *reinterpret_cast<u32x4_a2*>(p) = a;
+    return a;
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int nv, const float v[8]) {
-    if (nv >= 8) {
-        store8_full(p, v);
+
+// ---- eight elements of a row: which ones, and moving them ----------------------------------------------------------------
+// Columns of one lane's eight: col .. col + 3 and second .. second + 3.  Where everything is fp32 (SPLIT) the two quads lie apart,
+// so that neighbouring lanes take neighbouring 16 bytes in each access; else they are neighbours.
+struct Cols { uint32_t col, second; };            // unsigned: one 32-bit offset from a scalar row address
+
+template <typename T, bool SPLIT, bool NT>
+__device__ __forceinline__ Raw8<T> load_cols(const T* p, const Cols& c, int n_col, int n_second) {
+    Raw8<T> r;
+    if constexpr (sizeof(T) == 2) {
+        r.q[0] = load_raw<NT>(p + c.col, n_col);
+    } else {
+        // fp32 beside 16-bit rows: 32 bytes a lane, each line comes with two accesses, so it has to stay for the second
+        r.q[0] = load_raw<NT && SPLIT>(p + c.col, n_col);
+        r.q[1] = load_raw<NT && SPLIT>(p + c.second, SPLIT ? n_second : n_col - 4);
+    }
+    return r;
+}
+// n_col, n_second: elements of the row from col and second on (a 16-bit type looks at n_col alone)
+template <bool SPLIT, bool NT>
+__device__ __forceinline__ void store_cols(float* p, const Cols& c, int n_col, int n_second, const float v[8]) {
+    const int n[2] = {n_col, SPLIT ? n_second : n_col - 4};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float* q = p + (i ? c.second : c.col);
+        if (n[i] >= 4) {
+            put16<NT && SPLIT>(reinterpret_cast<u32x4_a2*>(q), pack4(v + 4 * i));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (e < n[i]) q[e] = v[4 * i + e];
+        }
+    }
+}
+template <bool SPLIT, bool NT, typename T>
+__device__ __forceinline__ void store_cols(T* p, const Cols& c, int n_col, int, const float v[8]) {
+    if (n_col >= 8) {
+        put16<NT>(reinterpret_cast<u32x4_a2*>(p + c.col), pack8(v, T{}));
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < nv) p[e] = from_f32<T>(v[e]);
+        for (int e = 0; e < 7; ++e)
+            if (e < n_col) p[c.col + e] = from_f32<T>(v[e]);
     }
+}
+// eight neighbours from column col on, nv of them in the row
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int col, int nv, float v[8]) {
+    unpack8(load_cols<T, false, false>(p, Cols{(uint32_t)col, (uint32_t)col + 4}, nv, nv - 4), v);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int col, int nv, const float v[8]) {
+    store_cols<false, false>(p, Cols{(uint32_t)col, (uint32_t)col + 4}, nv, nv - 4, v);
 }
 
 // ---- rows of a tensor whose leading axes have at most two strides: element (i, c) at (i / grp) * so + (i % grp) * si + c -----
@@ -116,7 +174,22 @@ struct Philox {
         return u32x4{a, b, c, d};
     }
 };
+// bit e: element e of the group is kept
+__device__ __forceinline__ uint32_t keep8(const Philox& ph, const DropoutArgs& a, uint32_t group, uint32_t row) {
+    const u32x4 w = ph.words(group, row);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t u = (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
+        bits |= u < a.threshold ? 0u : 1u << e;
+    }
+    return bits;
+}
 // v[e] <- kept ? v[e] * scale : 0.  A dropped infinity or NaN becomes 0: the element is replaced, not multiplied.
+__device__ __forceinline__ void drop8(uint32_t kept, float scale, float v[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = kept >> e & 1 ? v[e] * scale : 0.f;
+}
 __device__ __forceinline__ void drop8(const Philox& ph, const DropoutArgs& a, uint32_t group, uint32_t row, float v[8]) {
     const u32x4 w = ph.words(group, row);
 #pragma unroll

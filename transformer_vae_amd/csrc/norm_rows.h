@@ -1,0 +1,714 @@
+// The kernels of norms.hip, as templates: norms_f32.hip, norms_bf16.hip and norms_f16.hip compile them for x of their type.
+#pragma once
+#include "norm_common.h"
+
+namespace tvae {
+
+struct NormCall {
+    const void* x; const void* residual;            // at least one; T and R
+    RowsOf x_rows, res_rows;
+    int grp, d, groups;                             // groups = ceil(d / 8)
+    long long rows;
+    DropoutArgs drop;
+    const void* weight; const void* bias;           // null: 1 and 0
+    int w_f32, rms;                                 // weights are fp32 (else T); RMS norm
+    float eps, inv_d;                               // inv_d = 1 / d
+    float* mean; float* rstd;                       // forward: null in inference.  Backward: given (mean null for RMS)
+    void* y; void* sum;                             // forward outputs (T; R, nullable)
+    const void* dy; const void* dsum;               // backward: cotangents (T, nullable: 0; R, nullable: 0)
+    RowsOf dy_rows, ds_rows;
+    void* dx; void* dres;                           // nullable (T; R)
+    float* part; int chunks;                        // [2][chunks][d] partial sums of dw and db
+    int chunk_rows;
+    void* dw; void* db;                             // nullable
+};
+
+// one translation unit each
+int norm_launch_f32(const NormCall& c, bool bwd, hipStream_t s);
+int norm_launch_bf16(const NormCall& c, int r_dtype, bool bwd, hipStream_t s);
+int norm_launch_f16(const NormCall& c, int r_dtype, bool bwd, hipStream_t s);
+
+namespace {
+
+// sum over the 256 threads of a workgroup, the same bits in every thread
+__device__ __forceinline__ float block_sum(float v, float* sm) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (sm[0] + sm[1]) + (sm[2] + sm[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ void load8_param(const void* p, int f32, int col, int nv, float fill, float v[8]) {
+    if (!p) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fill;
+    } else if (f32) {
+        load8(static_cast<const float*>(p), col, nv, v);
+    } else {
+        load8(static_cast<const T*>(p), col, nv, v);
+    }
+}
+
+// the eight values of v that start at column 8 g; columns beyond d are 0
+template <typename T, typename R>
+__device__ __forceinline__ void value8(const NormCall& c, const Philox& ph, long long row, int g, float v[8]) {
+    const int nv = c.d - 8 * g;
+    if (c.x) {
+        load8(static_cast<const T*>(c.x) + row_offset(c.x_rows, c.grp, row), 8 * g, nv, v);
+        if (c.drop.threshold) drop8(ph, c.drop, (uint32_t)g, (uint32_t)row, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    }
+    if (c.residual) {
+        float r[8];
+        load8(static_cast<const R*>(c.residual) + row_offset(c.res_rows, c.grp, row), 8 * g, nv, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += r[e];
+    }
+}
+
+// ---- rows that fit the registers of TPR threads, V groups of eight columns each ----------------------------------------
+// Each of the inputs is read once: the row stays in registers between the sums and the output.  Rows of up to 512 elements
+// take 8 .. 64 lanes of a wave, so that several short rows share one; longer ones take whole waves and add their sums
+// through LDS.  The weights are loaded once a workgroup, which then walks over rows.
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// sum over aligned groups of LANES lanes, the same bits in each of them: exchanges inside rows of 16 lanes, then between
+// rows, all in the vector ALU
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v = dpp_add<0xB1>(v);                        // lane ^ 1
+    v = dpp_add<0x4E>(v);                        // lane ^ 2
+    v = dpp_add<0x141>(v);                       // the other four of eight
+    if constexpr (LANES >= 16) v = dpp_add<0x140>(v);
+    if constexpr (LANES >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (LANES >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
+// From four packs a thread on a row's loads alone fill the pipe: the next row's do not fly beside them, and the sums for dw and
+// db live in LDS, every thread's in places of its own.
+constexpr bool row_ahead(int v) { return v < 4; }
+
+template <int TPR>
+struct RowThreads {
+    static constexpr int BLOCK = TPR > 256 ? TPR : 256;
+    static constexpr int ROWS = BLOCK / TPR;             // rows a workgroup works on at a time
+    static constexpr int WAVES = TPR > 64 ? TPR / 64 : 1;  // waves of a row
+    static constexpr int WPE = 2;                        // waves a SIMD that the registers are held to
+};
+// sums of N values over the TPR threads of a row.  `sm` is one of two buffers that take turns, [BLOCK / 64][N]: a wave may
+// write the next sum while another still reads this one, and there is a barrier between this and the one after
+template <int TPR, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float* sm) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = lanes_sum<(TPR < 64 ? TPR : 64)>(v[i]);
+    if constexpr (TPR > 64) {
+        constexpr int W = RowThreads<TPR>::WAVES;
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) sm[wave * N + i] = v[i];
+        }
+        __syncthreads();
+        const float* mine = sm + (wave / W) * W * N;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float t = mine[i];
+#pragma unroll
+            for (int k = 1; k < W; ++k) t += mine[k * N + i];
+            v[i] = t;
+        }
+    }
+}
+
+// What a kernel is compiled for.  PLAIN: x alone, without dropout, dx alone.  FUSED: everything the call can ask for.  Both for
+// d that is a multiple of 8.  RAGGED: FUSED for other lengths, whose last elements are loaded and stored one by one.
+enum NormForm { PLAIN = 0, FUSED = 1, RAGGED = 2 };
+
+// the columns of a thread's pack k of eight, and how many of them are in the row
+template <int TPR, bool SPLIT, bool TAIL>
+struct RowCols {
+    uint32_t l, d;
+    __device__ __forceinline__ Cols at(int k) const {
+        if constexpr (SPLIT) return Cols{4 * (l + 2 * TPR * k), 4 * (l + 2 * TPR * k + TPR)};
+        else return Cols{8 * (l + TPR * k), 8 * (l + TPR * k) + 4};
+    }
+    __device__ __forceinline__ int left(uint32_t col) const { return (int)(d - col); }
+};
+
+// what one row's loads bring: those of a workgroup's next row fly while it works on this one
+template <typename T, int TPR, int V, bool SPLIT, bool TAIL, bool NT>
+struct RowLoad {
+    Raw8<T> g[V];
+    using C = RowCols<TPR, SPLIT, TAIL>;
+    __device__ __forceinline__ void get(const void* p, const RowsOf& rows, int grp, long long row, const C& cols) {
+        const T* q = static_cast<const T*>(p) + row_offset(rows, grp, row);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const Cols c = cols.at(k);
+            if constexpr (TAIL) {
+                g[k] = load_cols<T, SPLIT, NT>(q, c, cols.left(c.col), cols.left(c.second));
+            } else {
+                // every lane loads, those beyond the row its start, and use() takes zeros for them
+                const Cols in = {c.col < cols.d ? c.col : 0u, SPLIT ? (c.second < cols.d ? c.second : 0u) : (c.col < cols.d ? c.second : 4u)};
+                g[k] = load_cols<T, SPLIT, NT>(q, in, 8, 8);
+            }
+        }
+    }
+    __device__ __forceinline__ void use(int k, const C& cols, float v[8]) const {
+        Raw8<T> r = g[k];
+        if constexpr (!TAIL) {
+            const Cols c = cols.at(k);
+            const bool in = c.col < cols.d, in2 = SPLIT ? c.second < cols.d : in;
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r.q[i][e] = (i ? in2 : in) ? r.q[i][e] : 0u;
+        }
+        unpack8(r, v);
+    }
+};
+template <typename T, int TPR, bool SPLIT, bool TAIL, bool NT>
+__device__ __forceinline__ void store_pack(void* base, long long row, int k, const RowCols<TPR, SPLIT, TAIL>& cols, const float v[8]) {
+    T* p = static_cast<T*>(base) + row * cols.d;
+    const Cols c = cols.at(k);
+    if constexpr (TAIL) {
+        store_cols<SPLIT, NT>(p, c, cols.left(c.col), cols.left(c.second), v);
+    } else if constexpr (SPLIT) {
+        store_cols<true, NT>(p, c, c.col < cols.d ? 4 : 0, c.second < cols.d ? 4 : 0, v);
+    } else if (c.col < cols.d) {
+        store_cols<false, NT>(p, c, 8, 4, v);
+    }
+}
+// weights: `fill` where there are none, 0 beyond the row
+template <typename T, int TPR, bool SPLIT, bool TAIL>
+__device__ __forceinline__ void load_params(const void* p, int f32, int k, const RowCols<TPR, SPLIT, TAIL>& cols, float fill, float v[8]) {
+    const Cols c = cols.at(k);
+    if (!p) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fill;
+    } else if (SPLIT || f32) {
+        unpack8(load_cols<float, SPLIT, false>(static_cast<const float*>(p), c, cols.left(c.col), cols.left(c.second)), v);
+    } else {
+        unpack8(load_cols<T, SPLIT, false>(static_cast<const T*>(p), c, cols.left(c.col), cols.left(c.second)), v);
+    }
+}
+// keep decisions of a pack.  SPLIT: its quads are halves of two groups, whose other halves the neighbouring lane holds; each of the
+// two evaluates one of the groups and hands the other half over.
+template <int TPR, bool SPLIT, bool TAIL>
+__device__ __forceinline__ uint32_t keep_pack(const Philox& ph, const DropoutArgs& a, int k, const RowCols<TPR, SPLIT, TAIL>& cols, uint32_t row) {
+    if constexpr (!SPLIT) return keep8(ph, a, (uint32_t)(cols.l + TPR * k), row);
+    const int odd = cols.l & 1;
+    const uint32_t own = keep8(ph, a, (uint32_t)((cols.l >> 1) + TPR * k + (odd ? TPR / 2 : 0)), row);
+    const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)own, 0xB1, 0xf, 0xf, true);     // lane ^ 1
+    return odd ? (other >> 4) | (own & 0xf0u) : (own & 0xfu) | (other & 0xfu) << 4;
+}
+
+// The lane's columns as a turn of the row loop sees them: computed there from a value that the compiler cannot follow over the
+// loop, so that each access is a scalar row address with a 32-bit offset and not a 64-bit pointer a lane that stays in registers.
+template <int TPR, bool SPLIT, bool TAIL>
+__device__ __forceinline__ RowCols<TPR, SPLIT, TAIL> this_turn(RowCols<TPR, SPLIT, TAIL> cols) {
+    if constexpr (TPR >= 64) asm("" : "+v"(cols.l));
+    return cols;
+}
+
+template <int TPR>
+__device__ __forceinline__ int row_slot() {
+    if constexpr (TPR >= 64) return __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);     // one row a wave: scalar addresses
+    return threadIdx.x / TPR;
+}
+
+template <typename T, typename R, int TPR, int V, int FORM, bool NT>
+__global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void norm_fwd_kernel(NormCall c) {
+    using L = RowThreads<TPR>;
+    constexpr bool TAIL = FORM == RAGGED, SPLIT = sizeof(T) == 4;
+    __shared__ float sm[2][L::BLOCK / 64 * 2];
+    const Philox ph(c.drop);
+    const int sub = row_slot<TPR>();
+    const uint32_t l = threadIdx.x % TPR;
+    const RowCols<TPR, SPLIT, TAIL> cols0{l, (uint32_t)c.d};
+    const long long step = (long long)gridDim.x * L::ROWS;
+    long long row = (long long)blockIdx.x * L::ROWS + sub;
+    RowLoad<T, TPR, V, SPLIT, TAIL, NT> nx{};
+    RowLoad<R, TPR, V, SPLIT, TAIL, NT> nr{};
+    auto fetch = [&](long long at, const auto& cols) {
+        if (at >= c.rows) return;
+        if (FORM == PLAIN || c.x) nx.get(c.x, c.x_rows, c.grp, at, cols);
+        if (FORM != PLAIN && c.residual) nr.get(c.residual, c.res_rows, c.grp, at, cols);
+    };
+    if (row_ahead(V)) fetch(row, cols0);
+    float w[V][8], b[V][8];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        load_params<T>(c.weight, c.w_f32, k, cols0, 1.f, w[k]);
+        load_params<T>(c.bias, c.w_f32, k, cols0, 0.f, b[k]);
+    }
+    int turn = 0;
+    for (long long base = (long long)blockIdx.x * L::ROWS; base < c.rows; base += step, row += step) {
+        const auto cols = this_turn(cols0);
+        if (!row_ahead(V)) fetch(row, cols);
+        float v[V][8];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            nx.use(k, cols, v[k]);
+            if constexpr (FORM != PLAIN) {
+                if (c.x && c.drop.threshold) drop8(keep_pack(ph, c.drop, k, cols, (uint32_t)row), c.drop.scale, v[k]);
+                if (c.residual) {
+                    float r[8];
+                    nr.use(k, cols, r);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[k][e] += r[e];
+                }
+            }
+        }
+        if (row_ahead(V)) fetch(row + step, cols);
+        const bool live = row < c.rows;
+        if constexpr (FORM != PLAIN) {
+            if (c.sum && live) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) store_pack<R, TPR, SPLIT, TAIL, NT>(c.sum, row, k, cols, v[k]);
+            }
+        }
+        float mu = 0.f;
+        if (!c.rms) {
+            float s[1] = {0.f};
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                s[0] += ((v[k][0] + v[k][1]) + (v[k][2] + v[k][3])) + ((v[k][4] + v[k][5]) + (v[k][6] + v[k][7]));
+            row_sums<TPR, 1>(s, sm[turn]);
+            turn ^= 1;
+            mu = s[0] * c.inv_d;
+        }
+        // as in the kernel for any length: squares about the fp32 mean, and the mean of what is left
+        float q[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const Cols at = cols.at(k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t col = e < 4 ? at.col : at.second;
+                v[k][e] -= (TAIL ? col + (e & 3) : col) < cols.d ? mu : 0.f;
+                q[0] = fmaf(v[k][e], v[k][e], q[0]);
+                q[1] += v[k][e];
+            }
+        }
+        row_sums<TPR, 2>(q, sm[turn]);
+        turn ^= 1;
+        const float m2 = c.rms ? 0.f : q[1] * c.inv_d;
+        float var = q[0] * c.inv_d - m2 * m2;
+        if (var < 0.f) var = 0.f;
+        const float rs = rsqrtf(var + c.eps);
+        if (!live) continue;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] = fmaf((v[k][e] - m2) * rs, w[k][e], b[k][e]);
+            store_pack<T, TPR, SPLIT, TAIL, NT>(c.y, row, k, cols, v[k]);
+        }
+        if (l == 0 && c.rstd) {
+            c.rstd[row] = rs;
+            if (c.mean) c.mean[row] = mu + m2;
+        }
+    }
+}
+
+// The sums for dw and db grow in registers while the workgroup walks over rows; at the end the rows that a workgroup works on
+// at a time add theirs through LDS in a fixed order, and one partial sum a workgroup goes out.
+template <typename T, typename R, int TPR, int V, int FORM, bool NT>
+__global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void norm_bwd_kernel(NormCall c) {
+    using L = RowThreads<TPR>;
+    constexpr bool TAIL = FORM == RAGGED, SPLIT = sizeof(T) == 4;
+    __shared__ float sm[2][L::BLOCK / 64 * 2];
+    extern __shared__ float sums[];                  // [2][V][8][TPR] where the registers do not hold them
+    const Philox ph(c.drop);
+    const int sub = row_slot<TPR>();
+    const uint32_t l = threadIdx.x % TPR;
+    const RowCols<TPR, SPLIT, TAIL> cols0{l, (uint32_t)c.d};
+    const long long step = (long long)gridDim.x * L::ROWS;
+    long long row = (long long)blockIdx.x * L::ROWS + sub;
+    RowLoad<T, TPR, V, SPLIT, TAIL, NT> ny{}, nx{};
+    RowLoad<R, TPR, V, SPLIT, TAIL, NT> nr{};
+    float nmu = 0.f, nrs = 0.f;
+    auto fetch = [&](long long at, const auto& cols) {
+        if (at >= c.rows) return;
+        ny.get(c.dy, c.dy_rows, c.grp, at, cols);
+        if (FORM == PLAIN || c.x) nx.get(c.x, c.x_rows, c.grp, at, cols);
+        if (FORM != PLAIN && c.residual) nr.get(c.residual, c.res_rows, c.grp, at, cols);
+        nrs = c.rstd[at];
+        if (c.mean) nmu = c.mean[at];
+    };
+    if (row_ahead(V)) fetch(row, cols0);
+    float w[V][8], aw[V][8], ab[V][8];
+    auto slot = [&](int which, int k, int e) -> float& { return sums[((which * V + k) * 8 + e) * TPR + l]; };
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            aw[k][e] = 0.f; ab[k][e] = 0.f;
+            if (!row_ahead(V)) { slot(0, k, e) = 0.f; slot(1, k, e) = 0.f; }
+        }
+        load_params<T>(c.weight, c.w_f32, k, cols0, 1.f, w[k]);
+    }
+    int turn = 0;
+    for (long long base = (long long)blockIdx.x * L::ROWS; base < c.rows; base += step, row += step) {
+        const auto cols = this_turn(cols0);
+        const bool live = row < c.rows;
+        if (!row_ahead(V)) fetch(row, cols);
+        const float mu = nmu, rs = nrs;
+        float u[V][8], v[V][8];
+        uint32_t kept[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            nx.use(k, cols, v[k]);
+            if constexpr (FORM != PLAIN) {
+                kept[k] = 0;
+                if (c.drop.threshold) {
+                    kept[k] = keep_pack(ph, c.drop, k, cols, (uint32_t)row);
+                    if (c.x) drop8(kept[k], c.drop.scale, v[k]);
+                }
+                if (c.residual) {
+                    float r[8];
+                    nr.use(k, cols, r);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[k][e] += r[e];
+                }
+            }
+            ny.use(k, cols, u[k]);
+        }
+        RowLoad<R, TPR, V, SPLIT, TAIL, NT> ds{};        // before the next row's: loads arrive in order
+        if constexpr (FORM != PLAIN) {
+            if (c.dsum && live) ds.get(c.dsum, c.ds_rows, c.grp, row, cols);
+        }
+        if (row_ahead(V)) fetch(row + step, cols);
+        float s[2] = {0.f, 0.f};
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[k][e] = (v[k][e] - mu) * rs;
+                    if (row_ahead(V)) {
+                        aw[k][e] = fmaf(u[k][e], v[k][e], aw[k][e]);
+                        ab[k][e] += u[k][e];
+                    } else {
+                        slot(0, k, e) = fmaf(u[k][e], v[k][e], slot(0, k, e));
+                        slot(1, k, e) += u[k][e];
+                    }
+                    u[k][e] *= w[k][e];
+                    s[0] += u[k][e];
+                    s[1] = fmaf(u[k][e], v[k][e], s[1]);
+                }
+        }
+        row_sums<TPR, 2>(s, sm[turn]);
+        turn ^= 1;
+        if (!live || !(c.dx || (FORM != PLAIN && c.dres))) continue;
+        const float s1 = c.rms ? 0.f : s[0] * c.inv_d, s2 = s[1] * c.inv_d;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[k][e] = rs * ((u[k][e] - s1) - v[k][e] * s2);
+            if constexpr (FORM != PLAIN) {
+                if (c.dsum) {
+                    float t[8];
+                    ds.use(k, cols, t);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) u[k][e] += t[e];
+                }
+                if (c.dres) store_pack<R, TPR, SPLIT, TAIL, NT>(c.dres, row, k, cols, u[k]);
+                if (!c.dx) continue;
+                if (c.drop.threshold) drop8(kept[k], c.drop.scale, u[k]);
+            }
+            store_pack<T, TPR, SPLIT, TAIL, NT>(c.dx, row, k, cols, u[k]);
+        }
+    }
+    if (!c.part) return;
+    if constexpr (L::ROWS > 1) {
+        __shared__ float acc[L::ROWS - 1][TPR][9];      // nine: eight neighbouring words a lane would meet in eight banks
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                float (&a)[8] = which ? ab[k] : aw[k];
+                __syncthreads();
+                if (sub) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[sub - 1][l][e] = a[e];
+                }
+                __syncthreads();
+                if (!sub) {
+#pragma unroll 1
+                    for (int o = 0; o < L::ROWS - 1; ++o)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) a[e] += acc[o][l][e];
+                }
+            }
+    }
+    if (sub) return;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        if (!row_ahead(V)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { aw[k][e] = slot(0, k, e); ab[k][e] = slot(1, k, e); }
+        }
+        store_pack<float, TPR, SPLIT, TAIL, false>(c.part, blockIdx.x, k, cols0, aw[k]);
+        store_pack<float, TPR, SPLIT, TAIL, false>(c.part + (long long)c.chunks * c.d, blockIdx.x, k, cols0, ab[k]);
+    }
+}
+
+// ---- rows of any length: one workgroup per row, the row is read again for every pass over it ----------------------------
+template <typename T, typename R>
+__global__ __launch_bounds__(256) void norm_fwd_wide_kernel(NormCall c) {
+    __shared__ float sm[4];
+    const Philox ph(c.drop);
+    for (long long row = blockIdx.x; row < c.rows; row += gridDim.x) {
+        float mu = 0.f, m2 = 0.f, q = 0.f;
+        if (!c.rms) {
+            float s = 0.f;
+            for (int g = threadIdx.x; g < c.groups; g += 256) {
+                float v[8];
+                value8<T, R>(c, ph, row, g, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s += v[e];
+            }
+            mu = block_sum(s, sm) / (float)c.d;
+        }
+        // squares about the fp32 mean, with the sum of the deviations beside them: their mean is what rounding left in mu,
+        // and taking it out of both keeps rows of equal values at 0 under the smallest eps
+        float t1 = 0.f;
+        for (int g = threadIdx.x; g < c.groups; g += 256) {
+            float v[8];
+            value8<T, R>(c, ph, row, g, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float t = 8 * g + e < c.d ? v[e] - mu : 0.f;
+                t1 += t;
+                q = fmaf(t, t, q);
+            }
+        }
+        q = block_sum(q, sm) / (float)c.d;
+        if (!c.rms) {
+            m2 = block_sum(t1, sm) / (float)c.d;
+            q -= m2 * m2;
+            if (q < 0.f) q = 0.f;
+        }
+        const float rs = rsqrtf(q + c.eps);
+        for (int g = threadIdx.x; g < c.groups; g += 256) {
+            float v[8], w[8], b[8];
+            const int nv = c.d - 8 * g;
+            value8<T, R>(c, ph, row, g, v);
+            if (c.sum) store8(static_cast<R*>(c.sum) + row * c.d, 8 * g, nv, v);
+            load8_param<T>(c.weight, c.w_f32, 8 * g, nv, 1.f, w);
+            load8_param<T>(c.bias, c.w_f32, 8 * g, nv, 0.f, b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(((v[e] - mu) - m2) * rs, w[e], b[e]);
+            store8(static_cast<T*>(c.y) + row * c.d, 8 * g, nv, v);
+        }
+        if (threadIdx.x == 0 && c.rstd) {
+            c.rstd[row] = rs;
+            if (c.mean) c.mean[row] = mu + m2;
+        }
+    }
+}
+
+template <typename T, typename R>
+__global__ __launch_bounds__(256) void norm_bwd_wide_kernel(NormCall c) {
+    __shared__ float sm[4];
+    const Philox ph(c.drop);
+    for (long long row = blockIdx.x; row < c.rows; row += gridDim.x) {
+        const float mu = c.mean ? c.mean[row] : 0.f, rs = c.rstd[row];
+        const T* dy = static_cast<const T*>(c.dy) + row_offset(c.dy_rows, c.grp, row);
+        float s1 = 0.f, s2 = 0.f;
+        for (int g = threadIdx.x; g < c.groups; g += 256) {
+            float v[8], w[8], u[8];
+            const int nv = c.d - 8 * g;
+            value8<T, R>(c, ph, row, g, v);
+            load8(dy, 8 * g, nv, u);
+            load8_param<T>(c.weight, c.w_f32, 8 * g, nv, 1.f, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float gw = u[e] * w[e];
+                s1 += gw;
+                s2 = fmaf(gw, (v[e] - mu) * rs, s2);
+            }
+        }
+        s2 = block_sum(s2, sm) / (float)c.d;
+        s1 = c.rms ? 0.f : block_sum(s1, sm) / (float)c.d;
+        for (int g = threadIdx.x; g < c.groups; g += 256) {
+            float v[8], w[8], u[8];
+            const int nv = c.d - 8 * g;
+            value8<T, R>(c, ph, row, g, v);
+            load8(dy, 8 * g, nv, u);
+            load8_param<T>(c.weight, c.w_f32, 8 * g, nv, 1.f, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = rs * ((u[e] * w[e] - s1) - (v[e] - mu) * rs * s2);
+            if (c.dsum) {
+                load8(static_cast<const R*>(c.dsum) + row_offset(c.ds_rows, c.grp, row), 8 * g, nv, u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += u[e];
+            }
+            if (c.dres) store8(static_cast<R*>(c.dres) + row * c.d, 8 * g, nv, v);
+            if (c.dx) {
+                if (c.drop.threshold) drop8(ph, c.drop, (uint32_t)g, (uint32_t)row, v);
+                store8(static_cast<T*>(c.dx) + row * c.d, 8 * g, nv, v);
+            }
+        }
+    }
+}
+
+// partial sums of dw and db over chunk_rows rows: 64 groups of columns by 4 row lanes a workgroup
+template <typename T, typename R>
+__global__ __launch_bounds__(256) void norm_param_wide_kernel(NormCall c) {
+    __shared__ float sm[3][64][17];
+    const Philox ph(c.drop);
+    const int gl = threadIdx.x & 63, ry = threadIdx.x >> 6;
+    const int g = blockIdx.x * 64 + gl;
+    const long long r0 = (long long)blockIdx.y * c.chunk_rows, r1 = min(c.rows, r0 + c.chunk_rows);
+    float aw[8] = {}, ab[8] = {};
+    if (g < c.groups) {
+        for (long long row = r0 + ry; row < r1; row += 4) {
+            float v[8], u[8];
+            const float mu = c.mean ? c.mean[row] : 0.f, rs = c.rstd[row];
+            value8<T, R>(c, ph, row, g, v);
+            load8(static_cast<const T*>(c.dy) + row_offset(c.dy_rows, c.grp, row), 8 * g, c.d - 8 * g, u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                aw[e] = fmaf(u[e], (v[e] - mu) * rs, aw[e]);
+                ab[e] += u[e];
+            }
+        }
+    }
+    if (ry > 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { sm[ry - 1][gl][e] = aw[e]; sm[ry - 1][gl][8 + e] = ab[e]; }
+    }
+    __syncthreads();
+    if (ry == 0 && g < c.groups) {
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { aw[e] += sm[k][gl][e]; ab[e] += sm[k][gl][8 + e]; }
+        float* pw = c.part + (long long)blockIdx.y * c.d;
+        store8(pw, 8 * g, c.d - 8 * g, aw);
+        store8(pw + (long long)c.chunks * c.d, 8 * g, c.d - 8 * g, ab);
+    }
+}
+
+// ---- which kernel, and how many workgroups ----------------------------------------------------------------------------
+constexpr int NORM_CUS = 256;
+
+// threads a row and packs of eight a thread; tpr 0: the kernels for any length
+struct RowPlan { int tpr, v; };
+// the third list: where x and the residual are of 16 bits (three packs of fp32 do not fit the registers of a fused backward pass)
+#define NORM_SHAPES(X) X(8, 1) X(16, 1) X(32, 1) X(32, 2) X(64, 2) X(128, 2) X(256, 2) X(512, 2) X(512, 4)
+#define NORM_RAGGED_SHAPES(X) X(16, 1) X(32, 2) X(64, 2) X(256, 2) X(512, 4)
+#define NORM_NARROW_SHAPES(X) X(32, 3)
+inline RowPlan row_plan(int64_t d, bool narrow) {
+    const int64_t packs = (d + 7) / 8;
+    RowPlan p{0, 0};
+#define X(TPR, V) if (packs <= TPR * V && (!p.tpr || TPR * V < p.tpr * p.v)) p = RowPlan{TPR, V};
+    if (d % 8) { NORM_RAGGED_SHAPES(X) } else { NORM_SHAPES(X) }
+    if (d % 8 == 0 && narrow) { NORM_NARROW_SHAPES(X) }
+#undef X
+    return p;
+}
+inline NormForm norm_form(const NormCall& c) {
+    if (c.d % 8) return RAGGED;
+    return !c.x || c.residual || c.drop.threshold || c.sum || c.dsum || c.dres ? FUSED : PLAIN;
+}
+inline int plan_rows(const RowPlan& p) { return p.tpr >= 256 ? 1 : 256 / p.tpr; }
+inline int64_t plan_blocks(const RowPlan& p, bool bwd) { return (p.tpr > 256 ? 1 : p.v == 1 ? 4 : 2) * NORM_CUS; }
+inline bool norm_streams(const NormCall& c, int64_t esize) { return c.rows * c.d * esize >= (32ll << 20); }
+
+constexpr int64_t WIDE_CHUNK_ROWS = 64;          // rows a partial sum, at least; more where that would make over 1024 of them
+inline int64_t wide_chunk_rows(int64_t rows) {
+    const int64_t r = (rows + 1023) / 1024;
+    return r > WIDE_CHUNK_ROWS ? r : WIDE_CHUNK_ROWS;
+}
+// partial sums of a backward pass: workgroups of the row kernel, or chunks of rows
+inline int64_t bwd_chunks(int64_t rows, int64_t d, bool narrow) {
+    const RowPlan p = row_plan(d, narrow);
+    if (!p.tpr) { const int64_t r = wide_chunk_rows(rows); return (rows + r - 1) / r; }
+    const int64_t turns = (rows + plan_rows(p) - 1) / plan_rows(p), most = plan_blocks(p, true);
+    const int64_t want = (turns + 3) / 4;        // at least four turns a workgroup, while that leaves enough of them
+    const int64_t n = want < NORM_CUS ? (turns < NORM_CUS ? turns : NORM_CUS) : want;
+    return n < most ? n : most;
+}
+
+template <typename T, typename R, int TPR, int V, int FORM, bool NT>
+int norm_rows_launch(const NormCall& c, bool bwd, int64_t blocks, hipStream_t s) {
+    using L = RowThreads<TPR>;
+    size_t lds = 0;
+    if constexpr (!row_ahead(V)) {
+        if (bwd) {
+            lds = sizeof(float) * 2 * V * 8 * TPR;
+            static PerDeviceOnce once;
+            TVAE_CHECK_HIP(per_device_once(once, [] {
+                return hipFuncSetAttribute(reinterpret_cast<const void*>(&norm_bwd_kernel<T, R, TPR, V, FORM, NT>),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(float) * 2 * V * 8 * TPR));
+            }));
+        }
+    }
+    if (bwd) hipLaunchKernelGGL((norm_bwd_kernel<T, R, TPR, V, FORM, NT>), dim3((unsigned)blocks), dim3(L::BLOCK), lds, s, c);
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, R, TPR, V, FORM, NT>), dim3((unsigned)blocks), dim3(L::BLOCK), 0, s, c);
+    TVAE_CHECK_HIP(hipGetLastError());
+    return TVAE_OK;
+}
+template <typename T, typename R, int FORM, bool NT>
+int norm_rows(const RowPlan& p, const NormCall& c, bool bwd, int64_t blocks, hipStream_t s) {
+#define X(TPR, V) if (p.tpr == TPR && p.v == V) return norm_rows_launch<T, R, TPR, V, FORM, NT>(c, bwd, blocks, s);
+    if constexpr (FORM == RAGGED) { NORM_RAGGED_SHAPES(X) } else { NORM_SHAPES(X) }
+    if constexpr (FORM != RAGGED && sizeof(R) == 2) { NORM_NARROW_SHAPES(X) }
+#undef X
+    return fail(TVAE_ERR_ARG, "norm: no kernel for %d threads a row", p.tpr);
+}
+template <typename T, typename R>
+int norm_rows_form(const RowPlan& p, const NormCall& c, bool bwd, int64_t blocks, hipStream_t s) {
+    const NormForm form = norm_form(c);
+    const bool nt = norm_streams(c, sizeof(T));
+    if (form == RAGGED) return norm_rows<T, R, RAGGED, false>(p, c, bwd, blocks, s);
+    if (form == FUSED) return nt ? norm_rows<T, R, FUSED, true>(p, c, bwd, blocks, s) : norm_rows<T, R, FUSED, false>(p, c, bwd, blocks, s);
+    if constexpr (sizeof(T) == sizeof(R))
+        return nt ? norm_rows<T, T, PLAIN, true>(p, c, bwd, blocks, s) : norm_rows<T, T, PLAIN, false>(p, c, bwd, blocks, s);
+    return norm_rows_form<T, T>(p, c, bwd, blocks, s);          // nothing of the residual's type takes part
+}
+
+// forward, or the backward pass up to the partial sums (c.chunks = bwd_chunks, c.part null where dw and db are not wanted)
+template <typename T, typename R>
+int norm_launch(NormCall c, bool bwd, hipStream_t s) {
+    const RowPlan p = row_plan(c.d, sizeof(R) == 2);
+    if (p.tpr) {
+        const int64_t turns = (c.rows + plan_rows(p) - 1) / plan_rows(p), most = plan_blocks(p, bwd);
+        return norm_rows_form<T, R>(p, c, bwd, bwd ? c.chunks : turns < most ? turns : most, s);
+    }
+    const unsigned blocks = (unsigned)(c.rows < 65536 ? c.rows : 65536);
+    if (!bwd) {
+        hipLaunchKernelGGL((norm_fwd_wide_kernel<T, R>), dim3(blocks), dim3(256), 0, s, c);
+        TVAE_CHECK_HIP(hipGetLastError());
+        return TVAE_OK;
+    }
+    if (c.dx || c.dres) {
+        hipLaunchKernelGGL((norm_bwd_wide_kernel<T, R>), dim3(blocks), dim3(256), 0, s, c);
+        TVAE_CHECK_HIP(hipGetLastError());
+    }
+    if (c.part) {
+        c.chunk_rows = (int)wide_chunk_rows(c.rows);
+        hipLaunchKernelGGL((norm_param_wide_kernel<T, R>), dim3((unsigned)((c.groups + 63) / 64), (unsigned)c.chunks), dim3(256), 0, s, c);
+        TVAE_CHECK_HIP(hipGetLastError());
+    }
+    return TVAE_OK;
+}
+
+}  // namespace
+}  // namespace tvae
