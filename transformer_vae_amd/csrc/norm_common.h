@@ -24,23 +24,48 @@ __device__ __forceinline__ void put16(u32x4_a2* p, u32x4 v) {
 // eight elements in their type's own bits, which is what a load in flight keeps in registers
 template <typename T> struct Raw8 { u32x4 q[sizeof(T) / 2]; };
 
-// the first nv of four (fp32) or eight (16 bits) elements at p in 16 bytes; the others are 0
+// The first nv of four (fp32) or eight (16 bits) elements at p in 16 bytes; the others are 0.  The end of a row that is no whole
+// pack comes in pieces of four, two and one element: at most three accesses.
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+typedef uint32_t u32_a2 __attribute__((aligned(2)));
 template <bool NT>
 __device__ __forceinline__ u32x4 load_raw(const float* p, int nv) {
     if (nv >= 4) return load16<NT>(reinterpret_cast<const u32x4_a2*>(p));
     u32x4 q = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-        if (e < nv) q[e] = reinterpret_cast<const uint32_t*>(p)[e];
+    if (nv <= 0) return q;
+    if (nv & 2) {
+        const u32x2 a = *reinterpret_cast<const u32x2_a2*>(p);
+        q[0] = a[0]; q[1] = a[1];
+    }
+    if (nv & 1) {
+        const uint32_t a = reinterpret_cast<const uint32_t*>(p)[nv & 2];
+        if (nv & 2) q[2] = a;
+        else q[0] = a;
+    }
     return q;
 }
 template <bool NT, typename T>
 __device__ __forceinline__ u32x4 load_raw(const T* p, int nv) {
     if (nv >= 8) return load16<NT>(reinterpret_cast<const u32x4_a2*>(p));
     u32x4 q = {0, 0, 0, 0};
+    if (nv <= 0) return q;
+    if (nv & 4) {
+        const u32x2 a = *reinterpret_cast<const u32x2_a2*>(p);
+        q[0] = a[0]; q[1] = a[1];
+    }
+    if (nv & 2) {
+        const uint32_t a = *reinterpret_cast<const u32_a2*>(p + (nv & 4));
+        if (nv & 4) q[2] = a;
+        else q[0] = a;
+    }
+    if (nv & 1) {
+        const uint32_t a = reinterpret_cast<const uint16_t*>(p)[nv & 6];
+        const int at = nv >> 1;
 #pragma unroll
-    for (int e = 0; e < 7; ++e)
-        if (e < nv) q[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+        for (int e = 0; e < 4; ++e)
+            if (at == e) q[e] = a;
+    }
     return q;
 }
 __device__ __forceinline__ void unpack8(const Raw8<float>& r, float v[8]) {
@@ -98,6 +123,22 @@ __device__ __forceinline__ Raw8<T> load_cols(const T* p, const Cols& c, int n_co
     }
     return r;
 }
+__device__ __forceinline__ void store_part(float* p, int nv, u32x4 q) {         // nv < 4
+    if (nv <= 0) return;
+    if (nv & 2) *reinterpret_cast<u32x2_a2*>(p) = u32x2{q[0], q[1]};
+    if (nv & 1) reinterpret_cast<uint32_t*>(p)[nv & 2] = nv & 2 ? q[2] : q[0];
+}
+template <typename T>
+__device__ __forceinline__ void store_part(T* p, int nv, u32x4 q) {             // nv < 8
+    if (nv <= 0) return;
+    if (nv & 4) *reinterpret_cast<u32x2_a2*>(p) = u32x2{q[0], q[1]};
+    if (nv & 2) *reinterpret_cast<u32_a2*>(p + (nv & 4)) = nv & 4 ? q[2] : q[0];
+    if (nv & 1) {
+        const int at = nv >> 1;
+        const uint32_t a = at & 2 ? (at & 1 ? q[3] : q[2]) : (at & 1 ? q[1] : q[0]);
+        reinterpret_cast<uint16_t*>(p)[nv & 6] = (uint16_t)a;
+    }
+}
 // n_col, n_second: elements of the row from col and second on (a 16-bit type looks at n_col alone)
 template <bool SPLIT, bool NT>
 __device__ __forceinline__ void store_cols(float* p, const Cols& c, int n_col, int n_second, const float v[8]) {
@@ -105,24 +146,14 @@ __device__ __forceinline__ void store_cols(float* p, const Cols& c, int n_col, i
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         float* q = p + (i ? c.second : c.col);
-        if (n[i] >= 4) {
-            put16<NT && SPLIT>(reinterpret_cast<u32x4_a2*>(q), pack4(v + 4 * i));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 3; ++e)
-                if (e < n[i]) q[e] = v[4 * i + e];
-        }
+        if (n[i] >= 4) put16<NT && SPLIT>(reinterpret_cast<u32x4_a2*>(q), pack4(v + 4 * i));
+        else store_part(q, n[i], pack4(v + 4 * i));
     }
 }
 template <bool SPLIT, bool NT, typename T>
 __device__ __forceinline__ void store_cols(T* p, const Cols& c, int n_col, int, const float v[8]) {
-    if (n_col >= 8) {
-        put16<NT>(reinterpret_cast<u32x4_a2*>(p + c.col), pack8(v, T{}));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-            if (e < n_col) p[c.col + e] = from_f32<T>(v[e]);
-    }
+    if (n_col >= 8) put16<NT>(reinterpret_cast<u32x4_a2*>(p + c.col), pack8(v, T{}));
+    else store_part(p + c.col, n_col, pack8(v, T{}));
 }
 // eight neighbours from column col on, nv of them in the row
 template <typename T>
@@ -155,6 +186,7 @@ struct DropoutArgs {
     uint32_t threshold;         // round(65536 p): an element is dropped where its draw is below it; 0 = no dropout
     float scale;                // 65536 / (65536 - threshold); 0 where everything is dropped
 };
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) { return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96); }
 struct Philox {
     uint32_t k0, k1, c2, c3;
     __device__ __forceinline__ explicit Philox(const DropoutArgs& a) {
@@ -167,8 +199,8 @@ struct Philox {
 #pragma unroll
         for (int r = 0; r < 10; ++r) {
             const uint64_t p = (uint64_t)a * 0xD2511F53u, q = (uint64_t)c * 0xCD9E8D57u;
-            a = (uint32_t)(q >> 32) ^ b ^ x; b = (uint32_t)q;
-            c = (uint32_t)(p >> 32) ^ d ^ y; d = (uint32_t)p;
+            a = xor3((uint32_t)(q >> 32), b, x); b = (uint32_t)q;
+            c = xor3((uint32_t)(p >> 32), d, y); d = (uint32_t)p;
             x += 0x9E3779B9u; y += 0xBB67AE85u;
         }
         return u32x4{a, b, c, d};
