@@ -144,3 +144,10 @@ def test_backward_workspace_query(lib):
     assert q(1, 1) >= 8
     # the partial sums stay small next to the rows themselves
     assert q(245760, 1024) <= 245760 * 1024 * 2 // 16
+
+
+def test_missing_extension_is_an_error(monkeypatch, tmp_path):
+    monkeypatch.setattr(_lib, "_host", None)
+    monkeypatch.setattr(_lib, "HOST_PATH", str(tmp_path / "_host.so"))
+    with pytest.raises(RuntimeError, match="has not been built"):
+        F.layer_norm(torch.randn(2, 8))

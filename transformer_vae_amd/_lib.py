@@ -15,6 +15,7 @@ import threading
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libtvae_hip.so")
+HOST_PATH = os.path.join(_HERE, "_host.so")         # C++ autograd nodes over the library (csrc/host.cpp)
 HEADER = os.path.join(os.path.dirname(_HERE), "include", "tvae_hip.h")
 
 TVAE_F32, TVAE_BF16, TVAE_F32_STRICT = 0, 1, 2      # TVAE_F32_STRICT: tvae_mmd_* only (include/tvae_hip.h)
@@ -82,10 +83,11 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_host = None
 
 
 def build(force: bool = False) -> str:
-    """Compile csrc/*.hip into libtvae_hip.so for gfx950.  Works without a GPU."""
+    """Compile csrc/*.hip into libtvae_hip.so for gfx950 and csrc/host.cpp into _host.so.  Works without a GPU."""
     if force:
         subprocess.run(["make", "-C", CSRC, "clean"], check=True, capture_output=True)
     proc = subprocess.run(["make", "-C", CSRC, "-j4"], capture_output=True, text=True)
@@ -112,6 +114,20 @@ def lib() -> ctypes.CDLL:
                     fn.argtypes = args
                 _lib = handle
     return _lib
+
+
+def host():
+    """The module of C++ autograd nodes (loads on first use; raises if it has not been built)."""
+    global _host
+    if _host is None:
+        lib()
+        if not os.path.exists(HOST_PATH):
+            raise RuntimeError(f"{HOST_PATH} is missing: the extension has not been built "
+                               "(run `python -c 'import __graft_entry__ as g; g.build()'` or `make -C transformer_vae_amd/csrc`). "
+                               "There is no CPU fallback for this path.")
+        from . import _host as module
+        _host = module
+    return _host
 
 
 def check(status: int, what: str) -> None:

@@ -494,205 +494,6 @@ class _RbfKernel(torch.autograd.Function):
 
 
 # ------------------------------------------------------------------------------------------
-# norms and dropout of the sub-layers around the bottleneck (csrc/norms.hip, csrc/dropout.hip)
-# ------------------------------------------------------------------------------------------
-
-_ROW_DTYPES = {torch.float32: _lib.TVAE_F32, torch.bfloat16: _lib.TVAE_BF16, torch.float16: _lib.TVAE_F16}
-
-
-def _rows_of(what: str, tensors):
-    """Row layout of tensors of one shape (..., d): ([(tensor, so, si)], grp, rows, d), element (i, c) of a tensor at
-    (i // grp) * so + (i % grp) * si + c (include/tvae_hip.h).  Dense tensors, 2-d ones and 3-d ones of any row strides are
-    read where they lie (the first n tokens of longer sequences, an expanded batch); anything else is made dense first."""
-    shape = next(t.shape for t in tensors if t is not None)
-    d = shape[-1]
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
-    tensors = [t if t is None or (t.stride(-1) == 1 and t.dim() in (2, 3)) or t.is_contiguous() else t.contiguous() for t in tensors]
-    if all(t is None or t.is_contiguous() for t in tensors):
-        return [(t, d, 0) for t in tensors], 1, rows, d
-    if len(shape) == 2:
-        return [(t, 0 if t is None else t.stride(0), 0) for t in tensors], 1, rows, d
-    grp = shape[1]
-    return [(t, 0 if t is None else t.stride(0), 0 if t is None else t.stride(1)) for t in tensors], grp, rows, d
-
-
-def _row_args(r):
-    t, so, si = r
-    return _ptr(t), so, si
-
-
-def _rng_args(rng):
-    """(device pointer, seed, offset) of a call: `rng` is an int64 tensor {seed, offset} or a pair of ints or None."""
-    if rng is None:
-        return None, 0, 0
-    if isinstance(rng, torch.Tensor):
-        return _ptr(rng), 0, 0
-    return None, rng[0], rng[1]
-
-
-class _Dropout(torch.autograd.Function):
-    """out = [residual +] dropout(x); the mask is evaluated again in the backward pass, not stored."""
-
-    @staticmethod
-    def forward(ctx, x, residual, p: float, rng):
-        ctx.p, ctx.x_dtype = p, x.dtype
-        ctx.rng = None if isinstance(rng, torch.Tensor) else rng
-        ctx.save_for_backward(rng if isinstance(rng, torch.Tensor) else None)
-        return _dropout_launch(x, residual, p, rng, x.dtype if residual is None else residual.dtype)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        (rng,) = ctx.saved_tensors
-        dx = _dropout_launch(dout, None, ctx.p, ctx.rng if rng is None else rng, ctx.x_dtype) if ctx.needs_input_grad[0] else None
-        return dx, dout if ctx.needs_input_grad[1] else None, None, None
-
-
-@_on_tensor_device
-def _dropout_launch(x, residual, p, rng, out_dtype):
-    (xr, rr), grp, rows, d = _rows_of("dropout", (x, residual))
-    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    if rows * d > 0:
-        _lib.check(_lib.lib().tvae_dropout(*_row_args(xr), *_row_args(rr), grp, _ptr(out), rows, d, p, *_rng_args(rng),
-                                           _ROW_DTYPES[x.dtype], _ROW_DTYPES[out_dtype], _stream(x)), "tvae_dropout")
-    return out
-
-
-class _Norm(torch.autograd.Function):
-    """(norm(v), v or None) with v = [residual +] dropout(x), one node for the sum, the dropout and the norm."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, kind: int, eps: float, p: float, rng, return_sum: bool):
-        ctx.set_materialize_grads(False)
-        y, s, mean, rstd = _norm_forward(x, residual, weight, bias, kind, eps, p, rng, return_sum, True)
-        # The backward pass needs v in fp32: it forms it again from x and the residual, or reads the returned sum where that
-        # holds v as it is (fp32: 4 bytes an element for the 4 + 2 or 4 + 4 of x and residual).  A 16-bit sum would put its
-        # rounding into the weights' gradient.
-        kept = return_sum and s.dtype == torch.float32
-        ctx.save_for_backward(None if kept else x, s if kept else residual, weight, mean, rstd,
-                              rng if isinstance(rng, torch.Tensor) else None)
-        ctx.rng = None if isinstance(rng, torch.Tensor) else rng
-        ctx.meta = (x.shape, x.dtype, None if residual is None else residual.dtype, kind, p,
-                    None if bias is None else bias.dtype)
-        return (y, s) if return_sum else y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, ds=None):
-        x, residual, weight, mean, rstd, rng = ctx.saved_tensors
-        shape, x_dtype, r_dtype, kind, p, b_dtype = ctx.meta
-        rng = ctx.rng if rng is None else rng
-        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
-        if dy is None:                      # only the sum was used: the norm has no part in the gradient
-            dx = dr = None
-            if ds is not None:
-                dx = _dropout_launch(ds, None, p, rng, x_dtype) if need_x else None
-                dr = ds if need_r else None
-            return dx, dr, None, None, None, None, None, None, None
-        dx, dr, dw, db = _norm_backward(dy, ds, x, residual, weight, mean, rstd, rng, shape, x_dtype, r_dtype, b_dtype, kind, p,
-                                        need_x, need_r, need_w, need_b)
-        return dx, dr, dw, db, None, None, None, None, None
-
-
-@_on_tensor_device
-def _norm_forward(x, residual, weight, bias, kind, eps, p, rng, return_sum, stats):
-    (xr, rr), grp, rows, d = _rows_of("norm", (x, residual))
-    dev = x.device
-    r_dtype = x.dtype if residual is None else residual.dtype
-    w_dtype = x.dtype if weight is None and bias is None else (weight if weight is not None else bias).dtype
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    s = torch.empty(x.shape, dtype=r_dtype, device=dev) if return_sum else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if stats else None
-    mean = torch.empty(rows, dtype=torch.float32, device=dev) if stats and kind == _lib.TVAE_NORM_LAYER else None
-    if rows > 0:
-        weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-        _lib.check(_lib.lib().tvae_norm_fwd(kind, *_row_args(xr), *_row_args(rr), grp, _ptr(weight), _ptr(bias), eps, p,
-                                            *_rng_args(rng), _ptr(y), _ptr(s), _ptr(mean), _ptr(rstd), rows, d,
-                                            _ROW_DTYPES[x.dtype], _ROW_DTYPES[w_dtype], _ROW_DTYPES[r_dtype], _stream(x)), "tvae_norm_fwd")
-    return y, s, mean, rstd
-
-
-@_on_tensor_device
-def _norm_backward(dy, ds, x, residual, weight, mean, rstd, rng, shape, x_dtype, r_dtype, b_dtype, kind, p, need_x, need_r, need_w, need_b):
-    (yr, sr, xr, rr), grp, rows, d = _rows_of("norm", (dy, ds, x, residual))
-    dev = dy.device
-    r_type = x_dtype if r_dtype is None else r_dtype
-    w_type = weight.dtype if weight is not None else b_dtype if b_dtype is not None else x_dtype
-    # without dropout x and a residual of its type have one gradient
-    shared = need_x and need_r and p == 0.0 and r_type == x_dtype
-    dx = torch.empty(shape, dtype=x_dtype, device=dev) if need_x else None
-    dr = torch.empty(shape, dtype=r_type, device=dev) if need_r and not shared else None
-    dw = torch.empty(d, dtype=w_type, device=dev) if need_w else None
-    db = torch.empty(d, dtype=w_type, device=dev) if need_b else None
-    if rows == 0:
-        for t in (dw, db):
-            if t is not None:
-                t.zero_()
-    elif need_x or need_r or need_w or need_b:
-        lib = _lib.lib()
-        ws = _workspace(lib.tvae_norm_bwd_workspace_bytes(rows, d), dev) if need_w or need_b else None
-        weight = None if weight is None else weight.contiguous()
-        _lib.check(lib.tvae_norm_bwd(kind, *_row_args(yr), *_row_args(sr), *_row_args(xr), *_row_args(rr), grp, _ptr(weight),
-                                     _ptr(mean), _ptr(rstd), p, *_rng_args(rng), _ptr(dx), _ptr(dr), _ptr(dw), _ptr(db), rows, d,
-                                     _ROW_DTYPES[x_dtype], _ROW_DTYPES[w_type], _ROW_DTYPES[r_type], _ptr(ws),
-                                     0 if ws is None else ws.numel(), _stream(dy)), "tvae_norm_bwd")
-    return dx, dx if shared else dr, dw, db
-
-
-def _check_rows(what, x, **others):
-    _require_device(x, what)
-    if x.dim() < 1:
-        raise ValueError(f"{what} works on rows of the last axis, got a tensor without axes")
-    if x.dtype not in _ROW_DTYPES:
-        raise TypeError(f"{what} takes float32, bfloat16 or float16, got {x.dtype}")
-    for name, t in others.items():
-        if t is None:
-            continue
-        want = x.shape if name == "residual" else x.shape[-1:]
-        if t.shape != want:
-            raise ValueError(f"{what}: {name} must be {tuple(want)}, got {tuple(t.shape)}")
-        if t.device != x.device:
-            raise ValueError(f"{what}: {name} is on {t.device}, x on {x.device}")
-        if t.dtype not in (x.dtype, torch.float32):
-            raise TypeError(f"{what}: {name} must be {x.dtype} or float32, got {t.dtype}")
-
-
-def _check_dropout(what, x, p, rng):
-    """(p, rng) as the launches take them; draws where dropout is on and no state is given."""
-    p = float(p)
-    if not 0.0 <= p <= 1.0:
-        raise ValueError(f"{what}: p must be between 0 and 1, got {p}")
-    if p == 0.0:
-        return p, None
-    if rng is None:
-        return p, dropout_rng(x.device)
-    if isinstance(rng, torch.Tensor):
-        if rng.dtype != torch.int64 or tuple(rng.shape) != (2,) or not rng.is_contiguous() or rng.device != x.device:
-            raise ValueError(f"{what}: rng must be two contiguous int64 on {x.device} (seed, offset), got {tuple(rng.shape)} {rng.dtype} on {rng.device}")
-        return p, rng.detach()
-    seed, offset = rng
-    return p, (int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF)
-
-
-def _norm(what, kind, x, residual, weight, bias, eps, p, rng, return_sum):
-    _check_rows(what, x, residual=residual, weight=weight, bias=bias)
-    if x.shape[-1] == 0:
-        raise ValueError(f"{what}: the last axis is empty")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"{what}: weight and bias are of one type, got {weight.dtype} and {bias.dtype}")
-    eps = float(eps)
-    if not 0.0 <= eps < 1e30:
-        raise ValueError(f"{what}: eps must be a finite number >= 0, got {eps}")
-    p, rng = _check_dropout(what, x, p, rng)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias)):
-        return _Norm.apply(x, residual, weight, bias, kind, eps, p, rng, bool(return_sum))
-    y, s, _, _ = _norm_forward(x, residual, weight, bias, kind, eps, p, rng, return_sum, False)
-    return (y, s) if return_sum else y
-
-
-# ------------------------------------------------------------------------------------------
 # functional API used by the modules in autoencoders.py
 # ------------------------------------------------------------------------------------------
 
@@ -820,15 +621,19 @@ def _slerp(t1, t2, ratio):
     return out if dt == t1.dtype else out.to(t1.dtype)
 
 
+# Norms and dropout of the sub-layers around the bottleneck (csrc/norms.hip, csrc/dropout.hip).  Their autograd nodes and the
+# checks of their arguments are C++ (csrc/host.cpp); shapes and values raise ValueError, types TypeError.
+
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
-    """Layer norm over the last axis of ``x`` (float32, bfloat16 or float16), differentiable.  ``weight`` and ``bias`` are of
-    x's type or float32 (mixed precision) and may be missing; the result is of x's type, statistics and sums are fp32."""
-    return _norm("layer_norm", _lib.TVAE_NORM_LAYER, x, None, weight, bias, eps, 0.0, None, False)
+    """Layer norm over the last axis of ``x`` (float32, bfloat16 or float16), differentiable once.  ``weight`` and ``bias`` are
+    of x's type or float32 (mixed precision) and may be missing; the result is of x's type, statistics and sums are fp32.
+    Rows of any strides along up to two leading axes are read where they lie."""
+    return _lib.host().norm("layer_norm", _lib.TVAE_NORM_LAYER, x, None, weight, bias, eps, 0.0, None, False)
 
 
 def rms_norm(x, weight=None, eps: float = 1e-6):
     """``x * (mean(x^2) + eps)^-1/2 * weight`` over the last axis (T5's layer norm); types as ``layer_norm``."""
-    return _norm("rms_norm", _lib.TVAE_NORM_RMS, x, None, weight, None, eps, 0.0, None, False)
+    return _lib.host().norm("rms_norm", _lib.TVAE_NORM_RMS, x, None, weight, None, eps, 0.0, None, False)
 
 
 def dropout_rng(device, generator=None):
@@ -844,11 +649,7 @@ def dropout(x, p: float, rng=None):
     tensor (seed, offset) on x's device, as ``dropout_rng`` draws it, or a pair of ints; missing, one is drawn.  The tensor is
     read when the kernel runs and must keep its values until the backward pass.  ``p`` is in force as its nearest
     multiple of 2^-16, and the scale is that value's.  A dropped infinity or NaN is 0."""
-    _check_rows("dropout", x)
-    p, rng = _check_dropout("dropout", x, p, rng)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Dropout.apply(x, None, p, rng)
-    return _dropout_launch(x, None, p, rng, x.dtype)
+    return _lib.host().dropout(x, None, p, rng)
 
 
 def dropout_add(x, residual, p: float, rng=None):
@@ -856,20 +657,16 @@ def dropout_add(x, residual, p: float, rng=None):
     the residual's type."""
     if residual is None:
         raise ValueError("dropout_add: residual is missing")
-    _check_rows("dropout_add", x, residual=residual)
-    p, rng = _check_dropout("dropout_add", x, p, rng)
-    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad):
-        return _Dropout.apply(x, residual, p, rng)
-    return _dropout_launch(x, residual, p, rng, residual.dtype)
+    return _lib.host().dropout(x, residual, p, rng)
 
 
 def dropout_add_layer_norm(x, residual=None, weight=None, bias=None, eps: float = 1e-5, p: float = 0.0, rng=None,
                            return_sum: bool = False):
     """``layer_norm(residual + dropout(x, p, rng))`` in one pass (a post-norm sub-layer); with ``return_sum`` also the sum, in
     the residual's type (a pre-norm sub-layer hands it on).  The norm sees the sum before it is rounded to that type."""
-    return _norm("dropout_add_layer_norm", _lib.TVAE_NORM_LAYER, x, residual, weight, bias, eps, p, rng, return_sum)
+    return _lib.host().norm("dropout_add_layer_norm", _lib.TVAE_NORM_LAYER, x, residual, weight, bias, eps, p, rng, return_sum)
 
 
 def dropout_add_rms_norm(x, residual=None, weight=None, eps: float = 1e-6, p: float = 0.0, rng=None, return_sum: bool = False):
     """``rms_norm(residual + dropout(x, p, rng))`` in one pass; as ``dropout_add_layer_norm``."""
-    return _norm("dropout_add_rms_norm", _lib.TVAE_NORM_RMS, x, residual, weight, None, eps, p, rng, return_sum)
+    return _lib.host().norm("dropout_add_rms_norm", _lib.TVAE_NORM_RMS, x, residual, weight, None, eps, p, rng, return_sum)
