@@ -98,9 +98,10 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
-// From four packs a thread on a row's loads alone fill the pipe: the next row's do not fly beside them, and the sums for dw and
-// db live in LDS, every thread's in places of its own.
-constexpr bool row_ahead(int v) { return v < 4; }
+// Four packs a thread: the sums for dw and db live in LDS, every thread's in places of its own, and the next row's loads do not
+// fly beside the current row's work in a backward pass whose registers they would not fit (FUSED, fp32).
+constexpr bool sums_in_lds(int v) { return v >= 4; }
+template <typename T, int V, int FORM> constexpr bool bwd_ahead() { return V < 4 || (FORM == 0 && sizeof(T) == 2); }
 
 template <int TPR>
 struct RowThreads {
@@ -193,6 +194,11 @@ __device__ __forceinline__ void store_pack(void* base, long long row, int k, con
         store_cols<false, NT>(p, c, 8, 4, v);
     }
 }
+template <typename T, int TPR, bool SPLIT, bool TAIL>
+__device__ __forceinline__ void store_param(void* base, int f32, int k, const RowCols<TPR, SPLIT, TAIL>& cols, const float v[8]) {
+    if (SPLIT || f32) store_pack<float, TPR, SPLIT, TAIL, false>(base, 0, k, cols, v);
+    else store_pack<T, TPR, SPLIT, TAIL, false>(base, 0, k, cols, v);
+}
 // weights: `fill` where there are none, 0 beyond the row
 template <typename T, int TPR, bool SPLIT, bool TAIL>
 __device__ __forceinline__ void load_params(const void* p, int f32, int k, const RowCols<TPR, SPLIT, TAIL>& cols, float fill, float v[8]) {
@@ -249,7 +255,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
         if (FORM == PLAIN || c.x) nx.get(c.x, c.x_rows, c.grp, at, cols);
         if (FORM != PLAIN && c.residual) nr.get(c.residual, c.res_rows, c.grp, at, cols);
     };
-    if (row_ahead(V)) fetch(row, cols0);
+    fetch(row, cols0);
     float w[V][8], b[V][8];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
@@ -259,7 +265,6 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
     int turn = 0;
     for (long long base = (long long)blockIdx.x * L::ROWS; base < c.rows; base += step, row += step) {
         const auto cols = this_turn(cols0);
-        if (!row_ahead(V)) fetch(row, cols);
         float v[V][8];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -274,7 +279,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
                 }
             }
         }
-        if (row_ahead(V)) fetch(row + step, cols);
+        fetch(row + step, cols);
         const bool live = row < c.rows;
         if constexpr (FORM != PLAIN) {
             if (c.sum && live) {
@@ -292,7 +297,8 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
             turn ^= 1;
             mu = s[0] * c.inv_d;
         }
-        // as in the kernel for any length: squares about the fp32 mean, and the mean of what is left
+        // squares about the fp32 mean, with the sum of the deviations beside them: their mean is what rounding left in mu,
+        // and taking it out of both keeps rows of equal values at 0 under the smallest eps
         float q[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -330,7 +336,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 template <typename T, typename R, int TPR, int V, int FORM, bool NT>
 __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void norm_bwd_kernel(NormCall c) {
     using L = RowThreads<TPR>;
-    constexpr bool TAIL = FORM == RAGGED, SPLIT = sizeof(T) == 4;
+    constexpr bool TAIL = FORM == RAGGED, SPLIT = sizeof(T) == 4, AHEAD = bwd_ahead<T, V, FORM>();
     __shared__ float sm[2][L::BLOCK / 64 * 2];
     extern __shared__ float sums[];                  // [2][V][8][TPR] where the registers do not hold them
     const Philox ph(c.drop);
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
         nrs = c.rstd[at];
         if (c.mean) nmu = c.mean[at];
     };
-    if (row_ahead(V)) fetch(row, cols0);
+    if (AHEAD) fetch(row, cols0);
     float w[V][8], aw[V][8], ab[V][8];
     auto slot = [&](int which, int k, int e) -> float& { return sums[((which * V + k) * 8 + e) * TPR + l]; };
 #pragma unroll
@@ -358,7 +364,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             aw[k][e] = 0.f; ab[k][e] = 0.f;
-            if (!row_ahead(V)) { slot(0, k, e) = 0.f; slot(1, k, e) = 0.f; }
+            if (sums_in_lds(V)) { slot(0, k, e) = 0.f; slot(1, k, e) = 0.f; }
         }
         load_params<T>(c.weight, c.w_f32, k, cols0, 1.f, w[k]);
     }
@@ -366,7 +372,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
     for (long long base = (long long)blockIdx.x * L::ROWS; base < c.rows; base += step, row += step) {
         const auto cols = this_turn(cols0);
         const bool live = row < c.rows;
-        if (!row_ahead(V)) fetch(row, cols);
+        if (!AHEAD) fetch(row, cols);
         const float mu = nmu, rs = nrs;
         float u[V][8], v[V][8];
         uint32_t kept[V];
@@ -392,7 +398,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
         if constexpr (FORM != PLAIN) {
             if (c.dsum && live) ds.get(c.dsum, c.ds_rows, c.grp, row, cols);
         }
-        if (row_ahead(V)) fetch(row + step, cols);
+        if (AHEAD) fetch(row + step, cols);
         float s[2] = {0.f, 0.f};
         if (live) {
 #pragma unroll
@@ -400,7 +406,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     v[k][e] = (v[k][e] - mu) * rs;
-                    if (row_ahead(V)) {
+                    if (!sums_in_lds(V)) {
                         aw[k][e] = fmaf(u[k][e], v[k][e], aw[k][e]);
                         ab[k][e] += u[k][e];
                     } else {
@@ -434,7 +440,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
             store_pack<T, TPR, SPLIT, TAIL, NT>(c.dx, row, k, cols, u[k]);
         }
     }
-    if (!c.part) return;
+    if (!c.dw && !c.db) return;
     if constexpr (L::ROWS > 1) {
         __shared__ float acc[L::ROWS - 1][TPR][9];      // nine: eight neighbouring words a lane would meet in eight banks
 #pragma unroll
@@ -459,16 +465,21 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
     if (sub) return;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        if (!row_ahead(V)) {
+        if (sums_in_lds(V)) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) { aw[k][e] = slot(0, k, e); ab[k][e] = slot(1, k, e); }
         }
-        store_pack<float, TPR, SPLIT, TAIL, false>(c.part, blockIdx.x, k, cols0, aw[k]);
-        store_pack<float, TPR, SPLIT, TAIL, false>(c.part + (long long)c.chunks * c.d, blockIdx.x, k, cols0, ab[k]);
+        if (c.chunks == 1) {                             // a lone workgroup's sums are the gradients
+            if (c.dw) store_param<T>(c.dw, c.w_f32, k, cols0, aw[k]);
+            if (c.db) store_param<T>(c.db, c.w_f32, k, cols0, ab[k]);
+        } else {
+            if (c.dw) store_pack<float, TPR, SPLIT, TAIL, false>(c.part, blockIdx.x, k, cols0, aw[k]);
+            if (c.db) store_pack<float, TPR, SPLIT, TAIL, false>(c.part + (long long)c.chunks * c.d, blockIdx.x, k, cols0, ab[k]);
+        }
     }
 }
 
-// ---- rows of any length: one workgroup per row, the row is read again for every pass over it ----------------------------
+// ---- longer rows: one workgroup per row, the row is read again for every pass over it ----------------------------
 template <typename T, typename R>
 __global__ __launch_bounds__(256) void norm_fwd_wide_kernel(NormCall c) {
     __shared__ float sm[4];
@@ -476,17 +487,12 @@ __global__ __launch_bounds__(256) void norm_fwd_wide_kernel(NormCall c) {
     for (long long row = blockIdx.x; row < c.rows; row += gridDim.x) {
         float mu = 0.f, m2 = 0.f, q = 0.f;
         if (!c.rms) {
-            float s = 0.f;
-            for (int g = threadIdx.x; g < c.groups; g += 256) {
-                float v[8];
-                value8<T, R>(c, ph, row, g, v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s += v[e];
-            }
-            mu = block_sum(s, sm) / (float)c.d;
+            // a first guess of the mean from the row's first 2048 elements (these rows are longer): it is off by at most
+            // sqrt(d / 2048) standard deviations, so sums about it lose next to nothing, and the row is read twice, not three times
+            float v[8];
+            value8<T, R>(c, ph, row, threadIdx.x, v);
+            mu = block_sum(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])), sm) * (1.f / 2048.f);
         }
-        // squares about the fp32 mean, with the sum of the deviations beside them: their mean is what rounding left in mu,
-        // and taking it out of both keeps rows of equal values at 0 under the smallest eps
         float t1 = 0.f;
         for (int g = threadIdx.x; g < c.groups; g += 256) {
             float v[8];
@@ -608,7 +614,7 @@ __global__ __launch_bounds__(256) void norm_param_wide_kernel(NormCall c) {
 // ---- which kernel, and how many workgroups ----------------------------------------------------------------------------
 constexpr int NORM_CUS = 256;
 
-// threads a row and packs of eight a thread; tpr 0: the kernels for any length
+// threads a row and packs of eight a thread; tpr 0: longer than any of these
 struct RowPlan { int tpr, v; };
 // the third list: where x and the residual are of 16 bits (three packs of fp32 do not fit the registers of a fused backward pass)
 #define NORM_SHAPES(X) X(8, 1) X(16, 1) X(32, 1) X(32, 2) X(64, 2) X(128, 2) X(256, 2) X(512, 2) X(512, 4)
@@ -641,6 +647,8 @@ inline int64_t bwd_chunks(int64_t rows, int64_t d, bool narrow) {
     const RowPlan p = row_plan(d, narrow);
     if (!p.tpr) { const int64_t r = wide_chunk_rows(rows); return (rows + r - 1) / r; }
     const int64_t turns = (rows + plan_rows(p) - 1) / plan_rows(p), most = plan_blocks(p, true);
+    // a few short rows: one workgroup and no second kernel (1 x 1024 bf16: 6.0 -> 4.1 us; five turns, 40 x 512 fp32: 6.9 -> 8.6)
+    if (turns <= 2 && rows * d <= 32768) return 1;
     const int64_t want = (turns + 3) / 4;        // at least four turns a workgroup, while that leaves enough of them
     const int64_t n = want < NORM_CUS ? (turns < NORM_CUS ? turns : NORM_CUS) : want;
     return n < most ? n : most;
@@ -650,7 +658,7 @@ template <typename T, typename R, int TPR, int V, int FORM, bool NT>
 int norm_rows_launch(const NormCall& c, bool bwd, int64_t blocks, hipStream_t s) {
     using L = RowThreads<TPR>;
     size_t lds = 0;
-    if constexpr (!row_ahead(V)) {
+    if constexpr (sums_in_lds(V)) {
         if (bwd) {
             lds = sizeof(float) * 2 * V * 8 * TPR;
             static PerDeviceOnce once;
@@ -684,7 +692,7 @@ int norm_rows_form(const RowPlan& p, const NormCall& c, bool bwd, int64_t blocks
     return norm_rows_form<T, T>(p, c, bwd, blocks, s);          // nothing of the residual's type takes part
 }
 
-// forward, or the backward pass up to the partial sums (c.chunks = bwd_chunks, c.part null where dw and db are not wanted)
+// forward, or the backward pass up to the partial sums (c.chunks = bwd_chunks; one chunk of the row kernels: dw and db themselves)
 template <typename T, typename R>
 int norm_launch(NormCall c, bool bwd, hipStream_t s) {
     const RowPlan p = row_plan(c.d, sizeof(R) == 2);
@@ -702,7 +710,7 @@ int norm_launch(NormCall c, bool bwd, hipStream_t s) {
         hipLaunchKernelGGL((norm_bwd_wide_kernel<T, R>), dim3(blocks), dim3(256), 0, s, c);
         TVAE_CHECK_HIP(hipGetLastError());
     }
-    if (c.part) {
+    if (c.dw || c.db) {
         c.chunk_rows = (int)wide_chunk_rows(c.rows);
         hipLaunchKernelGGL((norm_param_wide_kernel<T, R>), dim3((unsigned)((c.groups + 63) / 64), (unsigned)c.chunks), dim3(256), 0, s, c);
         TVAE_CHECK_HIP(hipGetLastError());

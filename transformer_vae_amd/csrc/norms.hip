@@ -116,10 +116,10 @@ extern "C" int tvae_norm_bwd(int kind, const void* dy, int64_t dy_so, int64_t dy
                      (long long)workspace_bytes, (long long)tvae_norm_bwd_workspace_bytes(rows, d));
     c.weight = weight; c.mean = const_cast<float*>(mean); c.rstd = const_cast<float*>(rstd);
     c.dy = dy; c.dsum = dsum; c.dy_rows = RowsOf{dy_so, dy_si}; c.ds_rows = RowsOf{ds_so, ds_si};
-    c.dx = dx; c.dres = dresidual; c.dw = dweight; c.db = dbias; c.part = dweight || dbias ? static_cast<float*>(workspace) : nullptr;
+    c.dx = dx; c.dres = dresidual; c.dw = dweight; c.db = dbias; c.part = static_cast<float*>(workspace);
     c.chunks = (int)bwd_chunks(rows, d, r_dtype != TVAE_F32);
     hipStream_t s = static_cast<hipStream_t>(stream);
     TVAE_PROPAGATE(norm_dispatch(c, dtype, r_dtype, true, s));
-    if (!c.part) return TVAE_OK;
+    if (!(dweight || dbias) || (c.chunks == 1 && row_plan(d, r_dtype != TVAE_F32).tpr)) return TVAE_OK;
     return w_dtype == TVAE_F32 ? norm_params<float>(c, s) : w_dtype == TVAE_BF16 ? norm_params<bf16>(c, s) : norm_params<f16>(c, s);
 }
