@@ -101,7 +101,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // Four packs a thread: the sums for dw and db live in LDS, every thread's in places of its own, and the next row's loads do not
 // fly beside the current row's work in a backward pass whose registers they would not fit (FUSED, fp32).
 constexpr bool sums_in_lds(int v) { return v >= 4; }
-template <typename T, int V, int FORM> constexpr bool bwd_ahead() { return V < 4 || (FORM == 0 && sizeof(T) == 2); }
+template <typename T, int V, int FORM> constexpr bool bwd_ahead() { return V < 4 || (!(FORM & 1) && sizeof(T) == 2); }
 
 template <int TPR>
 struct RowThreads {
@@ -135,12 +135,15 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float* sm) {
     }
 }
 
-// What a kernel is compiled for.  PLAIN: x alone, without dropout, dx alone.  FUSED: everything the call can ask for.  Both for
-// d that is a multiple of 8.  RAGGED: FUSED for other lengths, whose last elements are loaded and stored one by one.
-enum NormForm { PLAIN = 0, FUSED = 1, RAGGED = 2 };
+// What a kernel is compiled for.  PLAIN: x alone, without dropout, dx alone.  FUSED: everything the call can ask for.  The ragged
+// ones take d that is no multiple of 8 (their handling of the cut pack, compiled into all, cost the others 3 to 15 %); TINY
+// is FUSED for rows of less than eight elements, which are loaded piece by piece.
+enum NormForm { PLAIN = 0, FUSED = 1, RAGGED_PLAIN = 2, RAGGED_FUSED = 3, TINY = 7 };
+constexpr bool is_fused(int form) { return form & 1; }
+constexpr bool is_ragged(int form) { return form & 2; }
 
 // the columns of a thread's pack k of eight, and how many of them are in the row
-template <int TPR, bool SPLIT, bool TAIL>
+template <int TPR, bool SPLIT, int FORM>
 struct RowCols {
     uint32_t l, d;
     __device__ __forceinline__ Cols at(int k) const {
@@ -150,58 +153,69 @@ struct RowCols {
     __device__ __forceinline__ int left(uint32_t col) const { return (int)(d - col); }
 };
 
-// what one row's loads bring: those of a workgroup's next row fly while it works on this one
-template <typename T, int TPR, int V, bool SPLIT, bool TAIL, bool NT>
+// the last n elements of 16 bytes to their start, zeros behind them (n <= 0: all zeros)
+template <typename T>
+__device__ __forceinline__ u32x4 last_first(u32x4 q, int n) {
+    if constexpr (sizeof(T) == 4) {
+        const int a = 4 - n;
+        if (a & 1) q = u32x4{q[1], q[2], q[3], 0};
+        if (a & 2) q = u32x4{q[2], q[3], 0, 0};
+    } else {
+        const int a = 8 - n;
+        if (a & 1) q = u32x4{q[0] >> 16 | q[1] << 16, q[1] >> 16 | q[2] << 16, q[2] >> 16 | q[3] << 16, q[3] >> 16};
+        if (a & 2) q = u32x4{q[1], q[2], q[3], 0};
+        if (a & 4) q = u32x4{q[2], q[3], 0, 0};
+    }
+    return q;
+}
+
+// What one row's loads bring: those of a workgroup's next row fly while it works on this one.  Every lane loads whole 16 bytes: a
+// pack that the row's end cuts, or that lies beyond it, takes the row's last 16, and use() puts its elements in place.
+template <typename T, int TPR, int V, bool SPLIT, int FORM, bool NT>
 struct RowLoad {
+    static constexpr int N = 16 / (int)sizeof(T);        // elements of 16 bytes
     Raw8<T> g[V];
-    using C = RowCols<TPR, SPLIT, TAIL>;
+    using C = RowCols<TPR, SPLIT, FORM>;
     __device__ __forceinline__ void get(const void* p, const RowsOf& rows, int grp, long long row, const C& cols) {
         const T* q = static_cast<const T*>(p) + row_offset(rows, grp, row);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const Cols c = cols.at(k);
-            if constexpr (TAIL) {
-                g[k] = load_cols<T, SPLIT, NT>(q, c, cols.left(c.col), cols.left(c.second));
-            } else {
-                // every lane loads, those beyond the row its start, and use() takes zeros for them
-                const Cols in = {c.col < cols.d ? c.col : 0u, SPLIT ? (c.second < cols.d ? c.second : 0u) : (c.col < cols.d ? c.second : 4u)};
-                g[k] = load_cols<T, SPLIT, NT>(q, in, 8, 8);
-            }
+            if constexpr (FORM == TINY) g[k] = load_cols<T, SPLIT, NT>(q, c, cols.left(c.col), cols.left(c.second));
+            else g[k] = load_cols<T, SPLIT, NT>(q, Cols{min(c.col, cols.d - N), min(c.second, cols.d - N)}, 8, 8);
         }
     }
     __device__ __forceinline__ void use(int k, const C& cols, float v[8]) const {
         Raw8<T> r = g[k];
-        if constexpr (!TAIL) {
+        if constexpr (FORM != TINY) {
             const Cols c = cols.at(k);
-            const bool in = c.col < cols.d, in2 = SPLIT ? c.second < cols.d : in;
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+                const int nv = cols.left(i ? c.second : c.col);
+                if (is_ragged(FORM) && nv > 0 && nv < N) r.q[i] = last_first<T>(r.q[i], nv);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r.q[i][e] = (i ? in2 : in) ? r.q[i][e] : 0u;
+                for (int e = 0; e < 4; ++e) r.q[i][e] = nv > 0 ? r.q[i][e] : 0u;
+            }
         }
         unpack8(r, v);
     }
 };
-template <typename T, int TPR, bool SPLIT, bool TAIL, bool NT>
-__device__ __forceinline__ void store_pack(void* base, long long row, int k, const RowCols<TPR, SPLIT, TAIL>& cols, const float v[8]) {
+template <typename T, int TPR, bool SPLIT, int FORM, bool NT>
+__device__ __forceinline__ void store_pack(void* base, long long row, int k, const RowCols<TPR, SPLIT, FORM>& cols, const float v[8]) {
     T* p = static_cast<T*>(base) + row * cols.d;
     const Cols c = cols.at(k);
-    if constexpr (TAIL) {
-        store_cols<SPLIT, NT>(p, c, cols.left(c.col), cols.left(c.second), v);
-    } else if constexpr (SPLIT) {
-        store_cols<true, NT>(p, c, c.col < cols.d ? 4 : 0, c.second < cols.d ? 4 : 0, v);
-    } else if (c.col < cols.d) {
-        store_cols<false, NT>(p, c, 8, 4, v);
-    }
+    if constexpr (is_ragged(FORM)) store_cols<SPLIT, NT>(p, c, cols.left(c.col), cols.left(c.second), v);
+    else if constexpr (SPLIT) store_cols<true, NT>(p, c, c.col < cols.d ? 4 : 0, c.second < cols.d ? 4 : 0, v);
+    else if (c.col < cols.d) store_cols<false, NT>(p, c, 8, 4, v);
 }
-template <typename T, int TPR, bool SPLIT, bool TAIL>
-__device__ __forceinline__ void store_param(void* base, int f32, int k, const RowCols<TPR, SPLIT, TAIL>& cols, const float v[8]) {
-    if (SPLIT || f32) store_pack<float, TPR, SPLIT, TAIL, false>(base, 0, k, cols, v);
-    else store_pack<T, TPR, SPLIT, TAIL, false>(base, 0, k, cols, v);
+template <typename T, int TPR, bool SPLIT, int FORM>
+__device__ __forceinline__ void store_param(void* base, int f32, int k, const RowCols<TPR, SPLIT, FORM>& cols, const float v[8]) {
+    if (SPLIT || f32) store_pack<float, TPR, SPLIT, FORM, false>(base, 0, k, cols, v);
+    else store_pack<T, TPR, SPLIT, FORM, false>(base, 0, k, cols, v);
 }
 // weights: `fill` where there are none, 0 beyond the row
-template <typename T, int TPR, bool SPLIT, bool TAIL>
-__device__ __forceinline__ void load_params(const void* p, int f32, int k, const RowCols<TPR, SPLIT, TAIL>& cols, float fill, float v[8]) {
+template <typename T, int TPR, bool SPLIT, int FORM>
+__device__ __forceinline__ void load_params(const void* p, int f32, int k, const RowCols<TPR, SPLIT, FORM>& cols, float fill, float v[8]) {
     const Cols c = cols.at(k);
     if (!p) {
 #pragma unroll
@@ -214,8 +228,8 @@ __device__ __forceinline__ void load_params(const void* p, int f32, int k, const
 }
 // keep decisions of a pack.  SPLIT: its quads are halves of two groups, whose other halves the neighbouring lane holds; each of the
 // two evaluates one of the groups and hands the other half over.
-template <int TPR, bool SPLIT, bool TAIL>
-__device__ __forceinline__ uint32_t keep_pack(const Philox& ph, const DropoutArgs& a, int k, const RowCols<TPR, SPLIT, TAIL>& cols, uint32_t row) {
+template <int TPR, bool SPLIT, int FORM>
+__device__ __forceinline__ uint32_t keep_pack(const Philox& ph, const DropoutArgs& a, int k, const RowCols<TPR, SPLIT, FORM>& cols, uint32_t row) {
     if constexpr (!SPLIT) return keep8(ph, a, (uint32_t)(cols.l + TPR * k), row);
     const int odd = cols.l & 1;
     const uint32_t own = keep8(ph, a, (uint32_t)((cols.l >> 1) + TPR * k + (odd ? TPR / 2 : 0)), row);
@@ -225,8 +239,8 @@ __device__ __forceinline__ uint32_t keep_pack(const Philox& ph, const DropoutArg
 
 // The lane's columns as a turn of the row loop sees them: computed there from a value that the compiler cannot follow over the
 // loop, so that each access is a scalar row address with a 32-bit offset and not a 64-bit pointer a lane that stays in registers.
-template <int TPR, bool SPLIT, bool TAIL>
-__device__ __forceinline__ RowCols<TPR, SPLIT, TAIL> this_turn(RowCols<TPR, SPLIT, TAIL> cols) {
+template <int TPR, bool SPLIT, int FORM>
+__device__ __forceinline__ RowCols<TPR, SPLIT, FORM> this_turn(RowCols<TPR, SPLIT, FORM> cols) {
     if constexpr (TPR >= 64) asm("" : "+v"(cols.l));
     return cols;
 }
@@ -240,20 +254,20 @@ __device__ __forceinline__ int row_slot() {
 template <typename T, typename R, int TPR, int V, int FORM, bool NT>
 __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void norm_fwd_kernel(NormCall c) {
     using L = RowThreads<TPR>;
-    constexpr bool TAIL = FORM == RAGGED, SPLIT = sizeof(T) == 4;
+    constexpr bool SPLIT = sizeof(T) == 4;
     __shared__ float sm[2][L::BLOCK / 64 * 2];
     const Philox ph(c.drop);
     const int sub = row_slot<TPR>();
     const uint32_t l = threadIdx.x % TPR;
-    const RowCols<TPR, SPLIT, TAIL> cols0{l, (uint32_t)c.d};
+    const RowCols<TPR, SPLIT, FORM> cols0{l, (uint32_t)c.d};
     const long long step = (long long)gridDim.x * L::ROWS;
     long long row = (long long)blockIdx.x * L::ROWS + sub;
-    RowLoad<T, TPR, V, SPLIT, TAIL, NT> nx{};
-    RowLoad<R, TPR, V, SPLIT, TAIL, NT> nr{};
+    RowLoad<T, TPR, V, SPLIT, FORM, NT> nx{};
+    RowLoad<R, TPR, V, SPLIT, FORM, NT> nr{};
     auto fetch = [&](long long at, const auto& cols) {
         if (at >= c.rows) return;
-        if (FORM == PLAIN || c.x) nx.get(c.x, c.x_rows, c.grp, at, cols);
-        if (FORM != PLAIN && c.residual) nr.get(c.residual, c.res_rows, c.grp, at, cols);
+        if (!is_fused(FORM) || c.x) nx.get(c.x, c.x_rows, c.grp, at, cols);
+        if (is_fused(FORM) && c.residual) nr.get(c.residual, c.res_rows, c.grp, at, cols);
     };
     fetch(row, cols0);
     float w[V][8], b[V][8];
@@ -269,7 +283,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             nx.use(k, cols, v[k]);
-            if constexpr (FORM != PLAIN) {
+            if constexpr (is_fused(FORM)) {
                 if (c.x && c.drop.threshold) drop8(keep_pack(ph, c.drop, k, cols, (uint32_t)row), c.drop.scale, v[k]);
                 if (c.residual) {
                     float r[8];
@@ -281,10 +295,10 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
         }
         fetch(row + step, cols);
         const bool live = row < c.rows;
-        if constexpr (FORM != PLAIN) {
+        if constexpr (is_fused(FORM)) {
             if (c.sum && live) {
 #pragma unroll
-                for (int k = 0; k < V; ++k) store_pack<R, TPR, SPLIT, TAIL, NT>(c.sum, row, k, cols, v[k]);
+                for (int k = 0; k < V; ++k) store_pack<R, TPR, SPLIT, FORM, NT>(c.sum, row, k, cols, v[k]);
             }
         }
         float mu = 0.f;
@@ -303,10 +317,16 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const Cols at = cols.at(k);
+            if constexpr (is_ragged(FORM)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] -= (e < 4 ? at.col : at.second) + (e & 3) < cols.d ? mu : 0.f;
+            } else {
+                const float m[2] = {at.col < cols.d ? mu : 0.f, at.second < cols.d ? mu : 0.f};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] -= m[e >> 2];
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t col = e < 4 ? at.col : at.second;
-                v[k][e] -= (TAIL ? col + (e & 3) : col) < cols.d ? mu : 0.f;
                 q[0] = fmaf(v[k][e], v[k][e], q[0]);
                 q[1] += v[k][e];
             }
@@ -322,7 +342,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
         for (int k = 0; k < V; ++k) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[k][e] = fmaf((v[k][e] - m2) * rs, w[k][e], b[k][e]);
-            store_pack<T, TPR, SPLIT, TAIL, NT>(c.y, row, k, cols, v[k]);
+            store_pack<T, TPR, SPLIT, FORM, NT>(c.y, row, k, cols, v[k]);
         }
         if (l == 0 && c.rstd) {
             c.rstd[row] = rs;
@@ -336,23 +356,23 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 template <typename T, typename R, int TPR, int V, int FORM, bool NT>
 __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void norm_bwd_kernel(NormCall c) {
     using L = RowThreads<TPR>;
-    constexpr bool TAIL = FORM == RAGGED, SPLIT = sizeof(T) == 4, AHEAD = bwd_ahead<T, V, FORM>();
+    constexpr bool SPLIT = sizeof(T) == 4, AHEAD = bwd_ahead<T, V, FORM>();
     __shared__ float sm[2][L::BLOCK / 64 * 2];
     extern __shared__ float sums[];                  // [2][V][8][TPR] where the registers do not hold them
     const Philox ph(c.drop);
     const int sub = row_slot<TPR>();
     const uint32_t l = threadIdx.x % TPR;
-    const RowCols<TPR, SPLIT, TAIL> cols0{l, (uint32_t)c.d};
+    const RowCols<TPR, SPLIT, FORM> cols0{l, (uint32_t)c.d};
     const long long step = (long long)gridDim.x * L::ROWS;
     long long row = (long long)blockIdx.x * L::ROWS + sub;
-    RowLoad<T, TPR, V, SPLIT, TAIL, NT> ny{}, nx{};
-    RowLoad<R, TPR, V, SPLIT, TAIL, NT> nr{};
+    RowLoad<T, TPR, V, SPLIT, FORM, NT> ny{}, nx{};
+    RowLoad<R, TPR, V, SPLIT, FORM, NT> nr{};
     float nmu = 0.f, nrs = 0.f;
     auto fetch = [&](long long at, const auto& cols) {
         if (at >= c.rows) return;
         ny.get(c.dy, c.dy_rows, c.grp, at, cols);
-        if (FORM == PLAIN || c.x) nx.get(c.x, c.x_rows, c.grp, at, cols);
-        if (FORM != PLAIN && c.residual) nr.get(c.residual, c.res_rows, c.grp, at, cols);
+        if (!is_fused(FORM) || c.x) nx.get(c.x, c.x_rows, c.grp, at, cols);
+        if (is_fused(FORM) && c.residual) nr.get(c.residual, c.res_rows, c.grp, at, cols);
         nrs = c.rstd[at];
         if (c.mean) nmu = c.mean[at];
     };
@@ -379,7 +399,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             nx.use(k, cols, v[k]);
-            if constexpr (FORM != PLAIN) {
+            if constexpr (is_fused(FORM)) {
                 kept[k] = 0;
                 if (c.drop.threshold) {
                     kept[k] = keep_pack(ph, c.drop, k, cols, (uint32_t)row);
@@ -394,8 +414,8 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
             }
             ny.use(k, cols, u[k]);
         }
-        RowLoad<R, TPR, V, SPLIT, TAIL, NT> ds{};        // before the next row's: loads arrive in order
-        if constexpr (FORM != PLAIN) {
+        RowLoad<R, TPR, V, SPLIT, FORM, NT> ds{};        // before the next row's: loads arrive in order
+        if constexpr (is_fused(FORM)) {
             if (c.dsum && live) ds.get(c.dsum, c.ds_rows, c.grp, row, cols);
         }
         if (AHEAD) fetch(row + step, cols);
@@ -420,24 +440,24 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
         }
         row_sums<TPR, 2>(s, sm[turn]);
         turn ^= 1;
-        if (!live || !(c.dx || (FORM != PLAIN && c.dres))) continue;
+        if (!live || !(c.dx || (is_fused(FORM) && c.dres))) continue;
         const float s1 = c.rms ? 0.f : s[0] * c.inv_d, s2 = s[1] * c.inv_d;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) u[k][e] = rs * ((u[k][e] - s1) - v[k][e] * s2);
-            if constexpr (FORM != PLAIN) {
+            if constexpr (is_fused(FORM)) {
                 if (c.dsum) {
                     float t[8];
                     ds.use(k, cols, t);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) u[k][e] += t[e];
                 }
-                if (c.dres) store_pack<R, TPR, SPLIT, TAIL, NT>(c.dres, row, k, cols, u[k]);
+                if (c.dres) store_pack<R, TPR, SPLIT, FORM, NT>(c.dres, row, k, cols, u[k]);
                 if (!c.dx) continue;
                 if (c.drop.threshold) drop8(kept[k], c.drop.scale, u[k]);
             }
-            store_pack<T, TPR, SPLIT, TAIL, NT>(c.dx, row, k, cols, u[k]);
+            store_pack<T, TPR, SPLIT, FORM, NT>(c.dx, row, k, cols, u[k]);
         }
     }
     if (!c.dw && !c.db) return;
@@ -473,8 +493,8 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
             if (c.dw) store_param<T>(c.dw, c.w_f32, k, cols0, aw[k]);
             if (c.db) store_param<T>(c.db, c.w_f32, k, cols0, ab[k]);
         } else {
-            if (c.dw) store_pack<float, TPR, SPLIT, TAIL, false>(c.part, blockIdx.x, k, cols0, aw[k]);
-            if (c.db) store_pack<float, TPR, SPLIT, TAIL, false>(c.part + (long long)c.chunks * c.d, blockIdx.x, k, cols0, ab[k]);
+            if (c.dw) store_pack<float, TPR, SPLIT, FORM, false>(c.part, blockIdx.x, k, cols0, aw[k]);
+            if (c.db) store_pack<float, TPR, SPLIT, FORM, false>(c.part + (long long)c.chunks * c.d, blockIdx.x, k, cols0, ab[k]);
         }
     }
 }
@@ -616,22 +636,24 @@ constexpr int NORM_CUS = 256;
 
 // threads a row and packs of eight a thread; tpr 0: longer than any of these
 struct RowPlan { int tpr, v; };
-// the third list: where x and the residual are of 16 bits (three packs of fp32 do not fit the registers of a fused backward pass)
+// the last list: where x and the residual are of 16 bits (three packs of fp32 do not fit the registers of a fused backward pass)
 #define NORM_SHAPES(X) X(8, 1) X(16, 1) X(32, 1) X(32, 2) X(64, 2) X(128, 2) X(256, 2) X(512, 2) X(512, 4)
-#define NORM_RAGGED_SHAPES(X) X(16, 1) X(32, 2) X(64, 2) X(256, 2) X(512, 4)
+#define NORM_TINY_SHAPES(X) X(8, 1)
 #define NORM_NARROW_SHAPES(X) X(32, 3)
 inline RowPlan row_plan(int64_t d, bool narrow) {
     const int64_t packs = (d + 7) / 8;
     RowPlan p{0, 0};
 #define X(TPR, V) if (packs <= TPR * V && (!p.tpr || TPR * V < p.tpr * p.v)) p = RowPlan{TPR, V};
-    if (d % 8) { NORM_RAGGED_SHAPES(X) } else { NORM_SHAPES(X) }
-    if (d % 8 == 0 && narrow) { NORM_NARROW_SHAPES(X) }
+    NORM_SHAPES(X)
+    if (narrow) { NORM_NARROW_SHAPES(X) }
 #undef X
     return p;
 }
 inline NormForm norm_form(const NormCall& c) {
-    if (c.d % 8) return RAGGED;
-    return !c.x || c.residual || c.drop.threshold || c.sum || c.dsum || c.dres ? FUSED : PLAIN;
+    if (c.d < 8) return TINY;
+    const bool fused = !c.x || c.residual || c.drop.threshold || c.sum || c.dsum || c.dres;
+    if (c.d % 8) return fused ? RAGGED_FUSED : RAGGED_PLAIN;
+    return fused ? FUSED : PLAIN;
 }
 inline int plan_rows(const RowPlan& p) { return p.tpr >= 256 ? 1 : 256 / p.tpr; }
 inline int64_t plan_blocks(const RowPlan& p, bool bwd) { return (p.tpr > 256 ? 1 : p.v == 1 ? 4 : 2) * NORM_CUS; }
@@ -676,8 +698,8 @@ int norm_rows_launch(const NormCall& c, bool bwd, int64_t blocks, hipStream_t s)
 template <typename T, typename R, int FORM, bool NT>
 int norm_rows(const RowPlan& p, const NormCall& c, bool bwd, int64_t blocks, hipStream_t s) {
 #define X(TPR, V) if (p.tpr == TPR && p.v == V) return norm_rows_launch<T, R, TPR, V, FORM, NT>(c, bwd, blocks, s);
-    if constexpr (FORM == RAGGED) { NORM_RAGGED_SHAPES(X) } else { NORM_SHAPES(X) }
-    if constexpr (FORM != RAGGED && sizeof(R) == 2) { NORM_NARROW_SHAPES(X) }
+    if constexpr (FORM == TINY) { NORM_TINY_SHAPES(X) } else { NORM_SHAPES(X) }
+    if constexpr (FORM != TINY && sizeof(R) == 2) { NORM_NARROW_SHAPES(X) }
 #undef X
     return fail(TVAE_ERR_ARG, "norm: no kernel for %d threads a row", p.tpr);
 }
@@ -685,11 +707,16 @@ template <typename T, typename R>
 int norm_rows_form(const RowPlan& p, const NormCall& c, bool bwd, int64_t blocks, hipStream_t s) {
     const NormForm form = norm_form(c);
     const bool nt = norm_streams(c, sizeof(T));
-    if (form == RAGGED) return norm_rows<T, R, RAGGED, false>(p, c, bwd, blocks, s);
-    if (form == FUSED) return nt ? norm_rows<T, R, FUSED, true>(p, c, bwd, blocks, s) : norm_rows<T, R, FUSED, false>(p, c, bwd, blocks, s);
-    if constexpr (sizeof(T) == sizeof(R))
-        return nt ? norm_rows<T, T, PLAIN, true>(p, c, bwd, blocks, s) : norm_rows<T, T, PLAIN, false>(p, c, bwd, blocks, s);
-    return norm_rows_form<T, T>(p, c, bwd, blocks, s);          // nothing of the residual's type takes part
+    switch (form) {
+        case TINY: return norm_rows<T, R, TINY, false>(p, c, bwd, blocks, s);
+        case RAGGED_FUSED: return norm_rows<T, R, RAGGED_FUSED, false>(p, c, bwd, blocks, s);
+        case FUSED: return nt ? norm_rows<T, R, FUSED, true>(p, c, bwd, blocks, s) : norm_rows<T, R, FUSED, false>(p, c, bwd, blocks, s);
+        default: break;
+    }
+    // nothing of the residual's type takes part
+    if constexpr (sizeof(T) != sizeof(R)) return norm_rows_form<T, T>(p, c, bwd, blocks, s);
+    else if (form == RAGGED_PLAIN) return norm_rows<T, T, RAGGED_PLAIN, false>(p, c, bwd, blocks, s);
+    else return nt ? norm_rows<T, T, PLAIN, true>(p, c, bwd, blocks, s) : norm_rows<T, T, PLAIN, false>(p, c, bwd, blocks, s);
 }
 
 // forward, or the backward pass up to the partial sums (c.chunks = bwd_chunks; one chunk of the row kernels: dw and db themselves)
