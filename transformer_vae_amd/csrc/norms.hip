@@ -15,27 +15,28 @@
 namespace tvae {
 namespace {
 
-// dw (blockIdx.y = 0) and db (1): the partial sums added in a fixed order, in fp64; 16 columns by 64 chunk lanes
-template <typename W>
+// dw, and db where blockIdx.y = 1 or there is no dw: the partial sums added in a fixed order, in fp64; COLS columns by
+// 1024 / COLS chunk lanes
+template <typename W, int COLS>
 __global__ __launch_bounds__(1024) void norm_param_final_kernel(const float* part, int chunks, int d, W* dw, W* db) {
-    __shared__ double sm[64][17];
-    W* out = blockIdx.y ? db : dw;
-    if (!out) return;
-    const float* p = part + (long long)blockIdx.y * chunks * d;
-    const int cx = threadIdx.x & 15, ry = threadIdx.x >> 4;
-    const long long col = (long long)blockIdx.x * 16 + cx;
+    constexpr int LANES = 1024 / COLS;
+    __shared__ double sm[LANES][COLS + 1];
+    const bool second = blockIdx.y || !dw;
+    W* out = second ? db : dw;
+    const float* p = part + (second ? (long long)chunks * d : 0);
+    const int cx = threadIdx.x % COLS, ry = threadIdx.x / COLS;
+    const long long col = (long long)blockIdx.x * COLS + cx;
     double s = 0.0;
     if (col < d) {
-#pragma unroll 4
-        for (int k = ry; k < chunks; k += 64) s += (double)p[(long long)k * d + col];
+#pragma unroll (COLS == 64 ? 8 : 4)
+        for (int k = ry; k < chunks; k += LANES) s += (double)p[(long long)k * d + col];
     }
     sm[ry][cx] = s;
     __syncthreads();
-    if (threadIdx.x < 256) {                     // 16 threads a column, four chunk lanes each
-        const int a = threadIdx.x >> 4;
-        sm[a][cx] = (sm[a][cx] + sm[a + 16][cx]) + (sm[a + 32][cx] + sm[a + 48][cx]);
+    if (LANES > 16) {                            // sixteen lanes a column take four each
+        if (ry < 16) sm[ry][cx] = (s + sm[ry + LANES / 4][cx]) + (sm[ry + LANES / 2][cx] + sm[ry + 3 * LANES / 4][cx]);
+        __syncthreads();
     }
-    __syncthreads();
     if (ry == 0 && col < d) {
         s = 0.0;
 #pragma unroll
@@ -49,10 +50,13 @@ int norm_dispatch(const NormCall& c, int dtype, int r_dtype, bool bwd, hipStream
     return dtype == TVAE_BF16 ? norm_launch_bf16(c, r_dtype, bwd, s) : norm_launch_f16(c, r_dtype, bwd, s);
 }
 
+// Long rows: 64 columns a workgroup, 256 bytes of every partial sum.  Short ones would leave most of the card idle then.
 template <typename W>
 int norm_params(const NormCall& c, hipStream_t s) {
-    hipLaunchKernelGGL((norm_param_final_kernel<W>), dim3((unsigned)((c.d + 15) / 16), 2), dim3(1024), 0, s, c.part, c.chunks, c.d,
-                       static_cast<W*>(c.dw), static_cast<W*>(c.db));
+    W *dw = static_cast<W*>(c.dw), *db = static_cast<W*>(c.db);
+    const unsigned both = dw && db ? 2 : 1;
+    if (c.d >= 8192) hipLaunchKernelGGL((norm_param_final_kernel<W, 64>), dim3((unsigned)((c.d + 63) / 64), both), dim3(1024), 0, s, c.part, c.chunks, c.d, dw, db);
+    else hipLaunchKernelGGL((norm_param_final_kernel<W, 16>), dim3((unsigned)((c.d + 15) / 16), both), dim3(1024), 0, s, c.part, c.chunks, c.d, dw, db);
     TVAE_CHECK_HIP(hipGetLastError());
     return TVAE_OK;
 }
