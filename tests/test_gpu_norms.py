@@ -173,6 +173,14 @@ def test_fused_types(d, x, w, r, rms):
         check((4 if d > 4096 else 21, d), x, w, r, rms, p, return_sum, seed=d + len(x))
 
 
+@pytest.mark.parametrize("x,w,r", [("f32", "f32", "f32"), ("bf16", "bf16", "bf16"), ("f16", "f32", "f32")])
+@pytest.mark.parametrize("d", [*range(1, 26), 517, 518, 519, 521, 1029, 1030, 1031, 1033, 16379, 16381, 16382, 16383])
+def test_cut_packs(d, x, w, r):
+    # every remainder of a pack of eight and of four, in the first pack and in later ones
+    check((3, d), x, w, r, d % 2 == 0, 0.1, True, seed=d)
+    check((3, d), x, w, "", d % 2 == 1, seed=d)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 31, 64, 65, 255, 257, 1025, 4099, 20011])
 def test_row_counts(rows):
     for d in (40, 768):

@@ -68,6 +68,17 @@ __device__ __forceinline__ u32x4 load_raw(const T* p, int nv) {
     }
     return q;
 }
+// the first nv of four 16-bit elements in 8 bytes
+template <bool NT, typename T>
+__device__ __forceinline__ u32x2 load_half(const T* p, int nv) {
+    if (nv >= 4) {
+        const u32x2_a2* q = reinterpret_cast<const u32x2_a2*>(p);
+        if constexpr (NT) return __builtin_nontemporal_load(q);
+        else return *q;
+    }
+    const u32x4 q = load_raw<false>(p, nv);
+    return u32x2{q[0], q[1]};
+}
 __device__ __forceinline__ void unpack8(const Raw8<float>& r, float v[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r.q[e >> 2][e & 3]);
@@ -107,17 +118,21 @@ __device__ __forceinline__ u32x4 pack8(const float v[8], f16) {
 }
 
 // ---- eight elements of a row: which ones, and moving them ----------------------------------------------------------------
-// Columns of one lane's eight: col .. col + 3 and second .. second + 3.  Where everything is fp32 (SPLIT) the two quads lie apart,
-// so that neighbouring lanes take neighbouring 16 bytes in each access; else they are neighbours.
+// Columns of one lane's eight: col .. col + 3 and second .. second + 3.  Where rows of fp32 take part (SPLIT) the two quads lie
+// apart, so that neighbouring lanes take neighbouring 16 bytes of them in each access (and 8 of 16-bit rows); else they are
+// neighbours.
 struct Cols { uint32_t col, second; };            // unsigned: one 32-bit offset from a scalar row address
 
 template <typename T, bool SPLIT, bool NT>
 __device__ __forceinline__ Raw8<T> load_cols(const T* p, const Cols& c, int n_col, int n_second) {
     Raw8<T> r;
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2 && SPLIT) {
+        const u32x2 a = load_half<NT>(p + c.col, n_col), b = load_half<NT>(p + c.second, n_second);
+        r.q[0] = u32x4{a[0], a[1], b[0], b[1]};
+    } else if constexpr (sizeof(T) == 2) {
         r.q[0] = load_raw<NT>(p + c.col, n_col);
     } else {
-        // fp32 beside 16-bit rows: 32 bytes a lane, each line comes with two accesses, so it has to stay for the second
+        // neighbouring quads: each line comes with two accesses, so it has to stay for the second
         r.q[0] = load_raw<NT && SPLIT>(p + c.col, n_col);
         r.q[1] = load_raw<NT && SPLIT>(p + c.second, SPLIT ? n_second : n_col - 4);
     }
@@ -139,7 +154,7 @@ __device__ __forceinline__ void store_part(T* p, int nv, u32x4 q) {             
         reinterpret_cast<uint16_t*>(p)[nv & 6] = (uint16_t)a;
     }
 }
-// n_col, n_second: elements of the row from col and second on (a 16-bit type looks at n_col alone)
+// n_col, n_second: elements of the row from col and second on (neighbouring quads: n_col says both)
 template <bool SPLIT, bool NT>
 __device__ __forceinline__ void store_cols(float* p, const Cols& c, int n_col, int n_second, const float v[8]) {
     const int n[2] = {n_col, SPLIT ? n_second : n_col - 4};
@@ -151,8 +166,19 @@ __device__ __forceinline__ void store_cols(float* p, const Cols& c, int n_col, i
     }
 }
 template <bool SPLIT, bool NT, typename T>
-__device__ __forceinline__ void store_cols(T* p, const Cols& c, int n_col, int, const float v[8]) {
-    if (n_col >= 8) put16<NT>(reinterpret_cast<u32x4_a2*>(p + c.col), pack8(v, T{}));
+__device__ __forceinline__ void store_cols(T* p, const Cols& c, int n_col, int n_second, const float v[8]) {
+    if constexpr (SPLIT) {
+        const u32x4 q = pack8(v, T{});
+        const int n[2] = {n_col, n_second};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            T* at = p + (i ? c.second : c.col);
+            const u32x2 h = {q[2 * i], q[2 * i + 1]};
+            if (n[i] < 4) store_part(at, n[i], u32x4{h[0], h[1], 0, 0});
+            else if constexpr (NT) __builtin_nontemporal_store(h, reinterpret_cast<u32x2_a2*>(at));
+            else *reinterpret_cast<u32x2_a2*>(at) = h;
+        }
+    } else if (n_col >= 8) put16<NT>(reinterpret_cast<u32x4_a2*>(p + c.col), pack8(v, T{}));
     else store_part(p + c.col, n_col, pack8(v, T{}));
 }
 // eight neighbours from column col on, nv of them in the row

@@ -153,27 +153,32 @@ struct RowCols {
     __device__ __forceinline__ int left(uint32_t col) const { return (int)(d - col); }
 };
 
-// the last n elements of 16 bytes to their start, zeros behind them (n <= 0: all zeros)
-template <typename T>
-__device__ __forceinline__ u32x4 last_first(u32x4 q, int n) {
-    if constexpr (sizeof(T) == 4) {
-        const int a = 4 - n;
-        if (a & 1) q = u32x4{q[1], q[2], q[3], 0};
-        if (a & 2) q = u32x4{q[2], q[3], 0, 0};
-    } else {
-        const int a = 8 - n;
-        if (a & 1) q = u32x4{q[0] >> 16 | q[1] << 16, q[1] >> 16 | q[2] << 16, q[2] >> 16 | q[3] << 16, q[3] >> 16};
-        if (a & 2) q = u32x4{q[1], q[2], q[3], 0};
-        if (a & 4) q = u32x4{q[2], q[3], 0, 0};
-    }
+// the last n elements of 16 bytes (of 8: the half that starts at dword h) to their start, zeros behind them
+__device__ __forceinline__ u32x4 last_first16(u32x4 q, int n) {          // eight 16-bit elements
+    const int a = 8 - n;
+    if (a & 1) q = u32x4{q[0] >> 16 | q[1] << 16, q[1] >> 16 | q[2] << 16, q[2] >> 16 | q[3] << 16, q[3] >> 16};
+    if (a & 2) q = u32x4{q[1], q[2], q[3], 0};
+    if (a & 4) q = u32x4{q[2], q[3], 0, 0};
+    return q;
+}
+__device__ __forceinline__ u32x4 last_first_half(u32x4 q, int h, int n) { // four 16-bit elements
+    const uint64_t v = ((uint64_t)q[h + 1] << 32 | q[h]) >> (16 * (4 - n));
+    q[h] = (uint32_t)v;
+    q[h + 1] = (uint32_t)(v >> 32);
+    return q;
+}
+__device__ __forceinline__ u32x4 last_first32(u32x4 q, int n) {          // four fp32 elements
+    const int a = 4 - n;
+    if (a & 1) q = u32x4{q[1], q[2], q[3], 0};
+    if (a & 2) q = u32x4{q[2], q[3], 0, 0};
     return q;
 }
 
-// What one row's loads bring: those of a workgroup's next row fly while it works on this one.  Every lane loads whole 16 bytes: a
-// pack that the row's end cuts, or that lies beyond it, takes the row's last 16, and use() puts its elements in place.
+// What one row's loads bring: those of a workgroup's next row fly while it works on this one.  Every access is whole: one that the
+// row's end cuts, or that lies beyond it, takes the row's last elements, and use() puts them in place.
 template <typename T, int TPR, int V, bool SPLIT, int FORM, bool NT>
 struct RowLoad {
-    static constexpr int N = 16 / (int)sizeof(T);        // elements of 16 bytes
+    static constexpr int N = SPLIT ? 4 : 8;              // elements of an access
     Raw8<T> g[V];
     using C = RowCols<TPR, SPLIT, FORM>;
     __device__ __forceinline__ void get(const void* p, const RowsOf& rows, int grp, long long row, const C& cols) {
@@ -189,12 +194,24 @@ struct RowLoad {
         Raw8<T> r = g[k];
         if constexpr (FORM != TINY) {
             const Cols c = cols.at(k);
+            const int n[2] = {cols.left(c.col), cols.left(c.second)};
+            if constexpr (sizeof(T) == 2 && !SPLIT) {
+                if (is_ragged(FORM) && n[0] > 0 && n[0] < 8) r.q[0] = last_first16(r.q[0], n[0]);
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-                const int nv = cols.left(i ? c.second : c.col);
-                if (is_ragged(FORM) && nv > 0 && nv < N) r.q[i] = last_first<T>(r.q[i], nv);
+                for (int e = 0; e < 4; ++e) r.q[0][e] = n[0] > 0 ? r.q[0][e] : 0u;
+            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r.q[i][e] = nv > 0 ? r.q[i][e] : 0u;
+                for (int i = 0; i < 2; ++i) {
+                    if constexpr (sizeof(T) == 2) {
+                        if (is_ragged(FORM) && n[i] > 0 && n[i] < 4) r.q[0] = last_first_half(r.q[0], 2 * i, n[i]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) r.q[0][2 * i + e] = n[i] > 0 ? r.q[0][2 * i + e] : 0u;
+                    } else {
+                        if (is_ragged(FORM) && n[i] > 0 && n[i] < 4) r.q[i] = last_first32(r.q[i], n[i]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) r.q[i][e] = n[i] > 0 ? r.q[i][e] : 0u;
+                    }
+                }
             }
         }
         unpack8(r, v);
@@ -210,7 +227,7 @@ __device__ __forceinline__ void store_pack(void* base, long long row, int k, con
 }
 template <typename T, int TPR, bool SPLIT, int FORM>
 __device__ __forceinline__ void store_param(void* base, int f32, int k, const RowCols<TPR, SPLIT, FORM>& cols, const float v[8]) {
-    if (SPLIT || f32) store_pack<float, TPR, SPLIT, FORM, false>(base, 0, k, cols, v);
+    if (sizeof(T) == 4 || f32) store_pack<float, TPR, SPLIT, FORM, false>(base, 0, k, cols, v);
     else store_pack<T, TPR, SPLIT, FORM, false>(base, 0, k, cols, v);
 }
 // weights: `fill` where there are none, 0 beyond the row
@@ -220,7 +237,7 @@ __device__ __forceinline__ void load_params(const void* p, int f32, int k, const
     if (!p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = fill;
-    } else if (SPLIT || f32) {
+    } else if (sizeof(T) == 4 || f32) {
         unpack8(load_cols<float, SPLIT, false>(static_cast<const float*>(p), c, cols.left(c.col), cols.left(c.second)), v);
     } else {
         unpack8(load_cols<T, SPLIT, false>(static_cast<const T*>(p), c, cols.left(c.col), cols.left(c.second)), v);
@@ -254,7 +271,7 @@ __device__ __forceinline__ int row_slot() {
 template <typename T, typename R, int TPR, int V, int FORM, bool NT>
 __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void norm_fwd_kernel(NormCall c) {
     using L = RowThreads<TPR>;
-    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr bool SPLIT = sizeof(R) == 4;
     __shared__ float sm[2][L::BLOCK / 64 * 2];
     const Philox ph(c.drop);
     const int sub = row_slot<TPR>();
@@ -356,7 +373,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 template <typename T, typename R, int TPR, int V, int FORM, bool NT>
 __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void norm_bwd_kernel(NormCall c) {
     using L = RowThreads<TPR>;
-    constexpr bool SPLIT = sizeof(T) == 4, AHEAD = bwd_ahead<T, V, FORM>();
+    constexpr bool SPLIT = sizeof(R) == 4, AHEAD = bwd_ahead<T, V, FORM>();
     __shared__ float sm[2][L::BLOCK / 64 * 2];
     extern __shared__ float sums[];                  // [2][V][8][TPR] where the registers do not hold them
     const Philox ph(c.drop);

@@ -19,7 +19,7 @@ namespace {
 // 1024 / COLS chunk lanes
 template <typename W, int COLS>
 __global__ __launch_bounds__(1024) void norm_param_final_kernel(const float* part, int chunks, int d, W* dw, W* db) {
-    constexpr int LANES = 1024 / COLS;
+    constexpr int LANES = 1024 / COLS, UNROLL = COLS == 64 ? 8 : 4;
     __shared__ double sm[LANES][COLS + 1];
     const bool second = blockIdx.y || !dw;
     W* out = second ? db : dw;
@@ -28,7 +28,7 @@ __global__ __launch_bounds__(1024) void norm_param_final_kernel(const float* par
     const long long col = (long long)blockIdx.x * COLS + cx;
     double s = 0.0;
     if (col < d) {
-#pragma unroll (COLS == 64 ? 8 : 4)
+#pragma unroll UNROLL
         for (int k = ry; k < chunks; k += LANES) s += (double)p[(long long)k * d + col];
     }
     sm[ry][cx] = s;
