@@ -200,25 +200,27 @@ def test_first_tokens_of_longer_sequences(d):
         check((6, 5, d), "bf16", "f32", "bf16", rms, 0.1, True, seq=7, seed=d)
 
 
-def test_layouts_give_the_same_bits():
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+def test_layouts_give_the_same_bits(x):
     g = torch.Generator(device=dev()).manual_seed(3)
-    for d in (77, 512):
-        base = torch.randn(4, 6, 2 * d, generator=g, device=dev())
+    t = TYPES[x]
+    for d in (7, 77, 512):
+        base = torch.randn(4, 6, 2 * d, generator=g, device=dev()).to(t)
         w, b = torch.randn(d, generator=g, device=dev()), torch.randn(d, generator=g, device=dev())
         layouts = [base[..., :d], base[..., 1:d + 1], base.transpose(0, 1)[..., :d], base[::2, 1:5, d:], base[:, :1, :d].expand(4, 9, d),
-                   torch.randn(d, 24, generator=g, device=dev()).t(), base.reshape(2, 2, 6, 2 * d)[:, :, 1:, :d], base[0, 0, :d]]
+                   torch.randn(d, 24, generator=g, device=dev()).to(t).t(), base.reshape(2, 2, 6, 2 * d)[:, :, 1:, :d], base[0, 0, :d]]
         for x in layouts:
-            dy = torch.randn(x.shape, generator=g, device=dev())
+            dy = torch.randn(x.shape, generator=g, device=dev()).to(t)
             got = []
-            for t in (x, x.contiguous()):
-                t = t.detach().requires_grad_(True)
-                y = F.dropout_add_layer_norm(t, dy, w, b, 1e-5, 0.1, (5, 6))
-                got.append((y, *torch.autograd.grad(y, t, dy), F.dropout(t, 0.3, (1, 2)), F.rms_norm(t, w)))
+            for v in (x, x.contiguous()):
+                v = v.detach().requires_grad_(True)
+                y = F.dropout_add_layer_norm(v, dy, w, b, 1e-5, 0.1, (5, 6))
+                got.append((y, *torch.autograd.grad(y, v, dy), F.dropout(v, 0.3, (1, 2)), F.rms_norm(v, w)))
             assert all(torch.equal(p, q) for p, q in zip(*got)), (d, x.shape, x.stride())
         # cotangents of other layouts: a slice, an expanded scalar, a transposed one
-        x = torch.randn(6, 4, d, generator=g, device=dev(), requires_grad=True)
+        x = torch.randn(6, 4, d, generator=g, device=dev()).to(t).requires_grad_(True)
         wg = w.clone().requires_grad_(True)
-        for dy in (base.transpose(0, 1)[..., :d], torch.ones((), device=dev()).expand(6, 4, d), base[..., ::2].transpose(0, 1)):
+        for dy in (base.transpose(0, 1)[..., :d], torch.ones((), device=dev(), dtype=t).expand(6, 4, d), base[..., ::2].transpose(0, 1)):
             y = F.rms_norm(x, wg)
             a = torch.autograd.grad(y, (x, wg), dy, retain_graph=True)
             c = torch.autograd.grad(y, (x, wg), dy.contiguous())
@@ -399,10 +401,11 @@ def test_second_derivatives_are_refused():
             g.sum().backward()
 
 
-def test_partial_gradients():
+@pytest.mark.parametrize("shape", [(5, 96), (33, 96), (1000, 300), (3, 20000)])
+def test_partial_gradients(shape):
     """Only the gradients that are asked for; each equals the one from asking for all."""
     for return_sum in (False, True):
-        xt, rt, wt, bt, dy, ds = make((33, 96), "bf16", "f32", "bf16", 4)
+        xt, rt, wt, bt, dy, ds = make(shape, "bf16", "f32", "bf16", 4)
         def run(need):
             ts = [t.detach().requires_grad_(k in need) for k, t in zip("xrwb", (xt, rt, wt, bt))]
             out = F.dropout_add_layer_norm(*ts, 1e-5, 0.1, (8, 8), return_sum)
@@ -527,6 +530,23 @@ def test_captured_steps_replay():
             want = step(*new)
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(got, want)), k
+
+
+def test_recomputed_forward_draws_the_same():
+    # activation checkpointing runs the forward pass again under the generator state that it saved
+    from torch.utils.checkpoint import checkpoint
+    w = torch.randn(64, device=dev(), requires_grad=True)
+    x = torch.randn(30, 64, device=dev(), requires_grad=True)
+
+    def block(t):
+        return F.dropout_add_rms_norm(t, t, w, p=0.3) + F.dropout(t, 0.5)
+
+    grads = []
+    for f in (block, lambda t: checkpoint(block, t, use_reentrant=False)):
+        torch.manual_seed(6)
+        y = f(x)
+        grads.append((y.detach(), *torch.autograd.grad(y.square().sum(), (x, w))))
+    assert all(torch.equal(p, q) for p, q in zip(*grads))
 
 
 def test_captured_dropout_draws_anew():

@@ -111,6 +111,8 @@ class LatentDecoderT5Norm(LatentDecoderNTokens):
     our kernels.  ``native_norm`` (or ``config.latent_decoder_native_norm``; always with a dropout rate): the block's
     norm, dropout and residual sum run on our kernels too, its two products stay where they are; same parameters."""
 
+    native_norm = False
+
     def __init__(self, config, dropout_rate=None, native_norm=None):
         super().__init__(config, dropout_rate)
         native = getattr(config, "latent_decoder_native_norm", False) if native_norm is None else native_norm

@@ -254,14 +254,6 @@ __device__ __forceinline__ uint32_t keep_pack(const Philox& ph, const DropoutArg
     return odd ? (other >> 4) | (own & 0xf0u) : (own & 0xfu) | (other & 0xfu) << 4;
 }
 
-// The lane's columns as a turn of the row loop sees them: computed there from a value that the compiler cannot follow over the
-// loop, so that each access is a scalar row address with a 32-bit offset and not a 64-bit pointer a lane that stays in registers.
-template <int TPR, bool SPLIT, int FORM>
-__device__ __forceinline__ RowCols<TPR, SPLIT, FORM> this_turn(RowCols<TPR, SPLIT, FORM> cols) {
-    if constexpr (TPR >= 64) asm("" : "+v"(cols.l));
-    return cols;
-}
-
 template <int TPR>
 __device__ __forceinline__ int row_slot() {
     if constexpr (TPR >= 64) return __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);     // one row a wave: scalar addresses
@@ -276,26 +268,25 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
     const Philox ph(c.drop);
     const int sub = row_slot<TPR>();
     const uint32_t l = threadIdx.x % TPR;
-    const RowCols<TPR, SPLIT, FORM> cols0{l, (uint32_t)c.d};
+    const RowCols<TPR, SPLIT, FORM> cols{l, (uint32_t)c.d};
     const long long step = (long long)gridDim.x * L::ROWS;
     long long row = (long long)blockIdx.x * L::ROWS + sub;
     RowLoad<T, TPR, V, SPLIT, FORM, NT> nx{};
     RowLoad<R, TPR, V, SPLIT, FORM, NT> nr{};
-    auto fetch = [&](long long at, const auto& cols) {
+    auto fetch = [&](long long at) {
         if (at >= c.rows) return;
         if (!is_fused(FORM) || c.x) nx.get(c.x, c.x_rows, c.grp, at, cols);
         if (is_fused(FORM) && c.residual) nr.get(c.residual, c.res_rows, c.grp, at, cols);
     };
-    fetch(row, cols0);
+    fetch(row);
     float w[V][8], b[V][8];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-        load_params<T>(c.weight, c.w_f32, k, cols0, 1.f, w[k]);
-        load_params<T>(c.bias, c.w_f32, k, cols0, 0.f, b[k]);
+        load_params<T>(c.weight, c.w_f32, k, cols, 1.f, w[k]);
+        load_params<T>(c.bias, c.w_f32, k, cols, 0.f, b[k]);
     }
     int turn = 0;
     for (long long base = (long long)blockIdx.x * L::ROWS; base < c.rows; base += step, row += step) {
-        const auto cols = this_turn(cols0);
         float v[V][8];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -310,7 +301,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
                 }
             }
         }
-        fetch(row + step, cols);
+        fetch(row + step);
         const bool live = row < c.rows;
         if constexpr (is_fused(FORM)) {
             if (c.sum && live) {
@@ -379,13 +370,13 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
     const Philox ph(c.drop);
     const int sub = row_slot<TPR>();
     const uint32_t l = threadIdx.x % TPR;
-    const RowCols<TPR, SPLIT, FORM> cols0{l, (uint32_t)c.d};
+    const RowCols<TPR, SPLIT, FORM> cols{l, (uint32_t)c.d};
     const long long step = (long long)gridDim.x * L::ROWS;
     long long row = (long long)blockIdx.x * L::ROWS + sub;
     RowLoad<T, TPR, V, SPLIT, FORM, NT> ny{}, nx{};
     RowLoad<R, TPR, V, SPLIT, FORM, NT> nr{};
     float nmu = 0.f, nrs = 0.f;
-    auto fetch = [&](long long at, const auto& cols) {
+    auto fetch = [&](long long at) {
         if (at >= c.rows) return;
         ny.get(c.dy, c.dy_rows, c.grp, at, cols);
         if (!is_fused(FORM) || c.x) nx.get(c.x, c.x_rows, c.grp, at, cols);
@@ -393,7 +384,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
         nrs = c.rstd[at];
         if (c.mean) nmu = c.mean[at];
     };
-    if (AHEAD) fetch(row, cols0);
+    if (AHEAD) fetch(row);
     float w[V][8], aw[V][8], ab[V][8];
     auto slot = [&](int which, int k, int e) -> float& { return sums[((which * V + k) * 8 + e) * TPR + l]; };
 #pragma unroll
@@ -403,13 +394,12 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
             aw[k][e] = 0.f; ab[k][e] = 0.f;
             if (sums_in_lds(V)) { slot(0, k, e) = 0.f; slot(1, k, e) = 0.f; }
         }
-        load_params<T>(c.weight, c.w_f32, k, cols0, 1.f, w[k]);
+        load_params<T>(c.weight, c.w_f32, k, cols, 1.f, w[k]);
     }
     int turn = 0;
     for (long long base = (long long)blockIdx.x * L::ROWS; base < c.rows; base += step, row += step) {
-        const auto cols = this_turn(cols0);
         const bool live = row < c.rows;
-        if (!AHEAD) fetch(row, cols);
+        if (!AHEAD) fetch(row);
         const float mu = nmu, rs = nrs;
         float u[V][8], v[V][8];
         uint32_t kept[V];
@@ -435,7 +425,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
         if constexpr (is_fused(FORM)) {
             if (c.dsum && live) ds.get(c.dsum, c.ds_rows, c.grp, row, cols);
         }
-        if (AHEAD) fetch(row + step, cols);
+        if (AHEAD) fetch(row + step);
         float s[2] = {0.f, 0.f};
         if (live) {
 #pragma unroll
@@ -507,11 +497,11 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
             for (int e = 0; e < 8; ++e) { aw[k][e] = slot(0, k, e); ab[k][e] = slot(1, k, e); }
         }
         if (c.chunks == 1) {                             // a lone workgroup's sums are the gradients
-            if (c.dw) store_param<T>(c.dw, c.w_f32, k, cols0, aw[k]);
-            if (c.db) store_param<T>(c.db, c.w_f32, k, cols0, ab[k]);
+            if (c.dw) store_param<T>(c.dw, c.w_f32, k, cols, aw[k]);
+            if (c.db) store_param<T>(c.db, c.w_f32, k, cols, ab[k]);
         } else {
-            if (c.dw) store_pack<float, TPR, SPLIT, FORM, false>(c.part, blockIdx.x, k, cols0, aw[k]);
-            if (c.db) store_pack<float, TPR, SPLIT, FORM, false>(c.part + (long long)c.chunks * c.d, blockIdx.x, k, cols0, ab[k]);
+            if (c.dw) store_pack<float, TPR, SPLIT, FORM, false>(c.part, blockIdx.x, k, cols, aw[k]);
+            if (c.db) store_pack<float, TPR, SPLIT, FORM, false>(c.part + (long long)c.chunks * c.d, blockIdx.x, k, cols, ab[k]);
         }
     }
 }
@@ -673,7 +663,12 @@ inline NormForm norm_form(const NormCall& c) {
     return fused ? FUSED : PLAIN;
 }
 inline int plan_rows(const RowPlan& p) { return p.tpr >= 256 ? 1 : 256 / p.tpr; }
-inline int64_t plan_blocks(const RowPlan& p, bool bwd) { return (p.tpr > 256 ? 1 : p.v == 1 ? 4 : 2) * NORM_CUS; }
+// Workgroups in flight, a CU: 512 threads of loads of two packs or more keep the memory busy, and the fewer streams there are, the
+// better the order in which it sees them (bf16, 245760 x 1024: forward 173 us with 512 workgroups of 256, 184 with 768, 190 with
+// 1024; backward 253 / 275 / 290).  Single packs need twice as many (fp32, 1000000 x 24: forward 61 us with two, 46 with four).
+inline int64_t plan_blocks(const RowPlan& p) { return (p.tpr > 256 ? 1 : p.v == 1 ? 4 : 2) * NORM_CUS; }
+// Streams of 32 MB on go past the caches (bf16, 245760 x 1024, backward: 280 -> 261 us); shorter ones may still be there when
+// the next kernel reads them (fp32, 5120 x 768, backward: 14.4 us with the caches, 16.5 past them).
 inline bool norm_streams(const NormCall& c, int64_t esize) { return c.rows * c.d * esize >= (32ll << 20); }
 
 constexpr int64_t WIDE_CHUNK_ROWS = 64;          // rows a partial sum, at least; more where that would make over 1024 of them
@@ -685,7 +680,7 @@ inline int64_t wide_chunk_rows(int64_t rows) {
 inline int64_t bwd_chunks(int64_t rows, int64_t d, bool narrow) {
     const RowPlan p = row_plan(d, narrow);
     if (!p.tpr) { const int64_t r = wide_chunk_rows(rows); return (rows + r - 1) / r; }
-    const int64_t turns = (rows + plan_rows(p) - 1) / plan_rows(p), most = plan_blocks(p, true);
+    const int64_t turns = (rows + plan_rows(p) - 1) / plan_rows(p), most = plan_blocks(p);
     // a few short rows: one workgroup and no second kernel (1 x 1024 bf16: 6.0 -> 4.1 us; five turns, 40 x 512 fp32: 6.9 -> 8.6)
     if (turns <= 2 && rows * d <= 32768) return 1;
     const int64_t want = (turns + 3) / 4;        // at least four turns a workgroup, while that leaves enough of them
@@ -741,7 +736,7 @@ template <typename T, typename R>
 int norm_launch(NormCall c, bool bwd, hipStream_t s) {
     const RowPlan p = row_plan(c.d, sizeof(R) == 2);
     if (p.tpr) {
-        const int64_t turns = (c.rows + plan_rows(p) - 1) / plan_rows(p), most = plan_blocks(p, bwd);
+        const int64_t turns = (c.rows + plan_rows(p) - 1) / plan_rows(p), most = plan_blocks(p);
         return norm_rows_form<T, R>(p, c, bwd, bwd ? c.chunks : turns < most ? turns : most, s);
     }
     const unsigned blocks = (unsigned)(c.rows < 65536 ? c.rows : 65536);
