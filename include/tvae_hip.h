@@ -328,7 +328,8 @@ int tvae_norm_fwd(int kind, const void* x, int64_t x_so, int64_t x_si, const voi
 /* Backward.  dy (rows, d) `dtype` with its own row strides; dsum (r_dtype, nullable) the cotangent of `sum`.
  * v is formed again from x and residual as in the forward call; a caller that kept an fp32 `sum` passes it as
  * `residual` with x NULL and the same p and rng (they still shape dx).  Outputs, all nullable and dense:
- * dx (`dtype`), dresidual (`r_dtype`), dweight and dbias (`w_dtype`).  The sums over rows have a fixed order. */
+ * dx (`dtype`), dresidual (`r_dtype`), dweight and dbias (`w_dtype`).  The sums over rows have a fixed order.
+ * workspace: for dweight and dbias, of the queried size (0 for small problems: it may be NULL then). */
 int64_t tvae_norm_bwd_workspace_bytes(int64_t rows, int64_t d);
 int tvae_norm_bwd(int kind, const void* dy, int64_t dy_so, int64_t dy_si, const void* dsum, int64_t ds_so, int64_t ds_si,
                   const void* x, int64_t x_so, int64_t x_si, const void* residual, int64_t res_so, int64_t res_si, int64_t grp,

@@ -120,7 +120,7 @@ def test_norm_fwd_refusals(lib, change, words):
 
 @pytest.mark.parametrize("change,words", [
     (dict(dy=None), "null pointer"), (dict(rstd=None), "null pointer"), (dict(mean=None), "needs mean"), (dict(kind=1), "neither"),
-    (dict(dw=P), "workspace"), (dict(dw=P, ws=P, nb=16), "workspace"), (dict(x=None), "null pointer"), (dict(t=1, rt=3), "residual"),
+    (dict(dw=P, rows=4000), "workspace"), (dict(dw=P, ws=P, nb=16, rows=4000), "workspace"), (dict(x=None), "null pointer"), (dict(t=1, rt=3), "residual"),
     (dict(p=2.0), "probability"), (dict(rows=6, grp=4), "groups"),
 ])
 def test_norm_bwd_refusals(lib, change, words):
@@ -141,7 +141,7 @@ def test_dropout_refusals(lib, change, words):
 def test_backward_workspace_query(lib):
     q = lib.tvae_norm_bwd_workspace_bytes
     assert q(0, 8) == q(8, 0) == q(1 << 31, 8) == q(8, 1 << 31) == -1
-    assert q(1, 1) >= 8
+    assert q(1, 1) == q(512, 2048) == 0 and q(513, 1) >= 8 and q(1, 2049) >= 2 * 4 * 2049
     # the partial sums stay small next to the rows themselves
     assert q(245760, 1024) <= 245760 * 1024 * 2 // 16
 

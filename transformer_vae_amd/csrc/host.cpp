@@ -274,13 +274,14 @@ struct NormNode : torch::autograd::Function<NormNode> {
                     if (need_b) db.zero_();
                 } else {
                     Tensor ws;
-                    if (need_w || need_b) ws = at::empty({tvae_norm_bwd_workspace_bytes(l.rows, l.d)}, dy.options().dtype(at::kByte));
+                    const int64_t bytes = need_w || need_b ? tvae_norm_bwd_workspace_bytes(l.rows, l.d) : 0;
+                    if (bytes > 0) ws = at::empty({bytes}, dy.options().dtype(at::kByte));
                     const Tensor weight = saved[2].defined() ? saved[2].contiguous() : saved[2];
                     check(tvae_norm_bwd((int)meta[4], ptr(l.r[0].t), l.r[0].so, l.r[0].si, ptr(l.r[1].t), l.r[1].so, l.r[1].si, ptr(l.r[2].t),
                                         l.r[2].so, l.r[2].si, ptr(l.r[3].t), l.r[3].so, l.r[3].si, l.grp, ptr(weight), (const float*)ptr(mean),
                                         (const float*)ptr(rstd), p, rng.device(), rng.seed, rng.offset, out_ptr(dx), out_ptr(dr), out_ptr(dw),
-                                        out_ptr(db), l.rows, l.d, code_of(x_type), code_of(w_type), code_of(r_type), out_ptr(ws),
-                                        ws.defined() ? ws.numel() : 0, stream_of(dy)), "tvae_norm_bwd");
+                                        out_ptr(db), l.rows, l.d, code_of(x_type), code_of(w_type), code_of(r_type), out_ptr(ws), bytes,
+                                        stream_of(dy)), "tvae_norm_bwd");
                 }
                 if (shared) dr = dx;
             }

@@ -225,11 +225,6 @@ __device__ __forceinline__ void store_pack(void* base, long long row, int k, con
     else if constexpr (SPLIT) store_cols<true, NT>(p, c, c.col < cols.d ? 4 : 0, c.second < cols.d ? 4 : 0, v);
     else if (c.col < cols.d) store_cols<false, NT>(p, c, 8, 4, v);
 }
-template <typename T, int TPR, bool SPLIT, int FORM>
-__device__ __forceinline__ void store_param(void* base, int f32, int k, const RowCols<TPR, SPLIT, FORM>& cols, const float v[8]) {
-    if (sizeof(T) == 4 || f32) store_pack<float, TPR, SPLIT, FORM, false>(base, 0, k, cols, v);
-    else store_pack<T, TPR, SPLIT, FORM, false>(base, 0, k, cols, v);
-}
 // weights: `fill` where there are none, 0 beyond the row
 template <typename T, int TPR, bool SPLIT, int FORM>
 __device__ __forceinline__ void load_params(const void* p, int f32, int k, const RowCols<TPR, SPLIT, FORM>& cols, float fill, float v[8]) {
@@ -496,14 +491,102 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 #pragma unroll
             for (int e = 0; e < 8; ++e) { aw[k][e] = slot(0, k, e); ab[k][e] = slot(1, k, e); }
         }
-        if (c.chunks == 1) {                             // a lone workgroup's sums are the gradients
-            if (c.dw) store_param<T>(c.dw, c.w_f32, k, cols, aw[k]);
-            if (c.db) store_param<T>(c.db, c.w_f32, k, cols, ab[k]);
-        } else {
-            if (c.dw) store_pack<float, TPR, SPLIT, FORM, false>(c.part, blockIdx.x, k, cols, aw[k]);
-            if (c.db) store_pack<float, TPR, SPLIT, FORM, false>(c.part + (long long)c.chunks * c.d, blockIdx.x, k, cols, ab[k]);
+        if (c.dw) store_pack<float, TPR, SPLIT, FORM, false>(c.part, blockIdx.x, k, cols, aw[k]);
+        if (c.db) store_pack<float, TPR, SPLIT, FORM, false>(c.part + (long long)c.chunks * c.d, blockIdx.x, k, cols, ab[k]);
+    }
+}
+
+// ---- a few hundred rows: dx, dw and db in one launch ------------------------------------------------------------------------
+// The first workgroups take a row a wave and write dx, the others take 16 columns each and write their dw and db: two packs by 128 row
+// lanes, whose sums meet in LDS in a fixed order.  Both read the inputs, which the caches hold at these sizes; what it saves is
+// the second kernel behind the first and the partial sums between them (fp32, one launch against two: 40 x 512 2.9 / 7.5 us,
+// 350 x 768 4.3 / 7.0, 512 x 2048 7.6 / 9.9; with dropout and residual 512 x 768 8.9 / 9.5: the row lanes' serial loops catch up).
+constexpr int SMALL_ROWS = 512, SMALL_D = 2048;
+inline bool bwd_small(int64_t rows, int64_t d) { return rows <= SMALL_ROWS && d <= SMALL_D; }
+
+template <typename T, typename R>
+__global__ __launch_bounds__(256) void norm_bwd_small_kernel(NormCall c, int row_blocks) {
+    const Philox ph(c.drop);
+    if ((int)blockIdx.x < row_blocks) {
+        constexpr int PACKS = SMALL_D / 8 / 64;
+        const int lane = threadIdx.x & 63;
+        const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+        if (row >= c.rows) return;
+        const float mu = c.mean ? c.mean[row] : 0.f, rs = c.rstd[row];
+        const T* dy = static_cast<const T*>(c.dy) + row_offset(c.dy_rows, c.grp, row);
+        float u[PACKS][8], v[PACKS][8], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            const int g = lane + 64 * k, nv = c.d - 8 * g;
+            if (g >= c.groups) continue;
+            float w[8];
+            load8(dy, 8 * g, nv, u[k]);
+            load8_param<T>(c.weight, c.w_f32, 8 * g, nv, 1.f, w);
+            value8<T, R>(c, ph, row, g, v[k]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[k][e] = (v[k][e] - mu) * rs;
+                u[k][e] *= w[e];
+                s1 += u[k][e];
+                s2 = fmaf(u[k][e], v[k][e], s2);
+            }
+        }
+        s1 = c.rms ? 0.f : lanes_sum<64>(s1) * c.inv_d;
+        s2 = lanes_sum<64>(s2) * c.inv_d;
+#pragma unroll
+        for (int k = 0; k < PACKS; ++k) {
+            const int g = lane + 64 * k, nv = c.d - 8 * g;
+            if (g >= c.groups) continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[k][e] = rs * ((u[k][e] - s1) - v[k][e] * s2);
+            if (c.dsum) {
+                float t[8];
+                load8(static_cast<const R*>(c.dsum) + row_offset(c.ds_rows, c.grp, row), 8 * g, nv, t);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[k][e] += t[e];
+            }
+            if (c.dres) store8(static_cast<R*>(c.dres) + row * c.d, 8 * g, nv, u[k]);
+            if (c.dx) {
+                if (c.drop.threshold) drop8(ph, c.drop, (uint32_t)g, (uint32_t)row, u[k]);
+                store8(static_cast<T*>(c.dx) + row * c.d, 8 * g, nv, u[k]);
+            }
+        }
+        return;
+    }
+    __shared__ float sums[2][128][18];           // 18: lanes that write eight neighbours meet few others in a bank
+    const int pack = threadIdx.x & 1, lane = threadIdx.x >> 1;
+    const int g = ((int)blockIdx.x - row_blocks) * 2 + pack;
+    float aw[8] = {}, ab[8] = {};
+    if (g < c.groups) {
+        for (long long row = lane; row < c.rows; row += 128) {
+            float u[8], v[8];
+            const float mu = c.mean ? c.mean[row] : 0.f, rs = c.rstd[row];
+            load8(static_cast<const T*>(c.dy) + row_offset(c.dy_rows, c.grp, row), 8 * g, c.d - 8 * g, u);
+            value8<T, R>(c, ph, row, g, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                aw[e] = fmaf(u[e], (v[e] - mu) * rs, aw[e]);
+                ab[e] += u[e];
+            }
         }
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { sums[0][lane][8 * pack + e] = aw[e]; sums[1][lane][8 * pack + e] = ab[e]; }
+    __syncthreads();
+    const int which = threadIdx.x >> 7, part = threadIdx.x >> 4 & 7, col = threadIdx.x & 15;     // eight threads a column
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += sums[which][16 * part + k][col];
+    __syncthreads();
+    sums[which][part][col] = t;
+    __syncthreads();
+    void* out = which ? c.db : c.dw;
+    const int at = ((int)blockIdx.x - row_blocks) * 16 + col;
+    if (part || at >= c.d || !out) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) t += sums[which][k][col];
+    if (sizeof(T) == 4 || c.w_f32) static_cast<float*>(out)[at] = t;
+    else static_cast<T*>(out)[at] = from_f32<T>(t);
 }
 
 // ---- longer rows: one workgroup per row, the row is read again for every pass over it ----------------------------
@@ -681,8 +764,6 @@ inline int64_t bwd_chunks(int64_t rows, int64_t d, bool narrow) {
     const RowPlan p = row_plan(d, narrow);
     if (!p.tpr) { const int64_t r = wide_chunk_rows(rows); return (rows + r - 1) / r; }
     const int64_t turns = (rows + plan_rows(p) - 1) / plan_rows(p), most = plan_blocks(p);
-    // a few short rows: one workgroup and no second kernel (1 x 1024 bf16: 6.0 -> 4.1 us; five turns, 40 x 512 fp32: 6.9 -> 8.6)
-    if (turns <= 2 && rows * d <= 32768) return 1;
     const int64_t want = (turns + 3) / 4;        // at least four turns a workgroup, while that leaves enough of them
     const int64_t n = want < NORM_CUS ? (turns < NORM_CUS ? turns : NORM_CUS) : want;
     return n < most ? n : most;
@@ -731,9 +812,15 @@ int norm_rows_form(const RowPlan& p, const NormCall& c, bool bwd, int64_t blocks
     else return nt ? norm_rows<T, T, PLAIN, true>(p, c, bwd, blocks, s) : norm_rows<T, T, PLAIN, false>(p, c, bwd, blocks, s);
 }
 
-// forward, or the backward pass up to the partial sums (c.chunks = bwd_chunks; one chunk of the row kernels: dw and db themselves)
+// forward, or the backward pass up to the partial sums (c.chunks = bwd_chunks)
 template <typename T, typename R>
 int norm_launch(NormCall c, bool bwd, hipStream_t s) {
+    if (bwd && (c.dw || c.db) && bwd_small(c.rows, c.d)) {
+        const int row_blocks = c.dx || c.dres ? (int)((c.rows + 3) / 4) : 0;
+        hipLaunchKernelGGL((norm_bwd_small_kernel<T, R>), dim3((unsigned)(row_blocks + (c.groups + 1) / 2)), dim3(256), 0, s, c, row_blocks);
+        TVAE_CHECK_HIP(hipGetLastError());
+        return TVAE_OK;
+    }
     const RowPlan p = row_plan(c.d, sizeof(R) == 2);
     if (p.tpr) {
         const int64_t turns = (c.rows + plan_rows(p) - 1) / plan_rows(p), most = plan_blocks(p);

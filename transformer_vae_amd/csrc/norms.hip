@@ -102,6 +102,7 @@ extern "C" int tvae_norm_fwd(int kind, const void* x, int64_t x_so, int64_t x_si
 
 extern "C" int64_t tvae_norm_bwd_workspace_bytes(int64_t rows, int64_t d) {
     if (rows <= 0 || d <= 0 || rows >= (1ll << 31) || d >= (1ll << 31)) return -1;
+    if (bwd_small(rows, d)) return 0;
     return 2 * std::max(bwd_chunks(rows, d, false), bwd_chunks(rows, d, true)) * d * 4;
 }
 
@@ -115,7 +116,7 @@ extern "C" int tvae_norm_bwd(int kind, const void* dy, int64_t dy_so, int64_t dy
     TVAE_REQUIRE(dy && rstd, "norm_bwd: null pointer argument");
     TVAE_REQUIRE(c.rms ? !mean && !dbias : mean != nullptr, "norm_bwd: layer norm needs mean, RMS norm has neither mean nor bias");
     if (!(dx || dresidual || dweight || dbias)) return TVAE_OK;
-    if (dweight || dbias)
+    if ((dweight || dbias) && !bwd_small(rows, d))
         TVAE_REQUIRE(workspace && workspace_bytes >= tvae_norm_bwd_workspace_bytes(rows, d), "norm_bwd: workspace of %lld bytes, %lld needed",
                      (long long)workspace_bytes, (long long)tvae_norm_bwd_workspace_bytes(rows, d));
     c.weight = weight; c.mean = const_cast<float*>(mean); c.rstd = const_cast<float*>(rstd);
@@ -124,6 +125,6 @@ extern "C" int tvae_norm_bwd(int kind, const void* dy, int64_t dy_so, int64_t dy
     c.chunks = (int)bwd_chunks(rows, d, r_dtype != TVAE_F32);
     hipStream_t s = static_cast<hipStream_t>(stream);
     TVAE_PROPAGATE(norm_dispatch(c, dtype, r_dtype, true, s));
-    if (!(dweight || dbias) || (c.chunks == 1 && row_plan(d, r_dtype != TVAE_F32).tpr)) return TVAE_OK;
+    if (!(dweight || dbias) || bwd_small(rows, d)) return TVAE_OK;
     return w_dtype == TVAE_F32 ? norm_params<float>(c, s) : w_dtype == TVAE_BF16 ? norm_params<bf16>(c, s) : norm_params<f16>(c, s);
 }
