@@ -103,6 +103,21 @@ __device__ __forceinline__ float lanes_sum(float v) {
 constexpr bool sums_in_lds(int v) { return v >= 4; }
 template <typename T, int V, int FORM> constexpr bool bwd_ahead() { return V < 4 || (!(FORM & 1) && sizeof(T) == 2); }
 
+// sum over the lanes of a wave that hold the same columns: those TPR apart
+template <int TPR>
+__device__ __forceinline__ float same_columns_sum(float v) {
+    if constexpr (TPR <= 8) v = dpp_add<0x128>(v);       // the other eight of sixteen
+    if constexpr (TPR <= 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (TPR <= 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
 template <int TPR>
 struct RowThreads {
     static constexpr int BLOCK = TPR > 256 ? TPR : 256;
@@ -355,7 +370,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
 }
 
 // The sums for dw and db grow in registers while the workgroup walks over rows; at the end the rows that a workgroup works on
-// at a time add theirs through LDS in a fixed order, and one partial sum a workgroup goes out.
+// at a time add theirs in a fixed order, across lanes and then through LDS, and one partial sum a workgroup goes out.
 template <typename T, typename R, int TPR, int V, int FORM, bool NT>
 __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void norm_bwd_kernel(NormCall c) {
     using L = RowThreads<TPR>;
@@ -463,28 +478,33 @@ __global__ __launch_bounds__(RowThreads<TPR>::BLOCK, RowThreads<TPR>::WPE) void 
         }
     }
     if (!c.dw && !c.db) return;
-    if constexpr (L::ROWS > 1) {
-        __shared__ float acc[L::ROWS - 1][TPR][9];      // nine: eight neighbouring words a lane would meet in eight banks
+    constexpr int SLOTS = TPR > 64 ? L::ROWS : 4;        // what is left to add once a wave's rows are one
+    const int slot_at = TPR > 64 ? sub : (int)(threadIdx.x >> 6);
+    if constexpr (SLOTS > 1) {
+        __shared__ float acc[SLOTS - 1][TPR][9];         // nine: eight neighbouring words a lane would meet in eight banks
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
+                if (!(which ? c.db : c.dw)) continue;
                 float (&a)[8] = which ? ab[k] : aw[k];
-                __syncthreads();
-                if (sub) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) acc[sub - 1][l][e] = a[e];
+                for (int e = 0; e < 8; ++e) a[e] = same_columns_sum<TPR>(a[e]);
+                __syncthreads();
+                if (slot_at && (threadIdx.x & 63) < TPR) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[slot_at - 1][l][e] = a[e];
                 }
                 __syncthreads();
-                if (!sub) {
-#pragma unroll 1
-                    for (int o = 0; o < L::ROWS - 1; ++o)
+                if (!slot_at) {
+#pragma unroll
+                    for (int o = 0; o < SLOTS - 1; ++o)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) a[e] += acc[o][l][e];
                 }
             }
     }
-    if (sub) return;
+    if (sub) return;                                     // (the first row's threads hold the sums)
 #pragma unroll
     for (int k = 0; k < V; ++k) {
         if (sums_in_lds(V)) {
