@@ -152,8 +152,8 @@ def check(shape, x, w, r="", rms=False, p=0.0, return_sum=False, seq=None, eps=1
 
 # lengths: one element, below / at / above a group of eight, the widths that models have, odd ones, and each side of the
 # places where another kernel or another number of lanes takes over
-LENGTHS = [1, 2, 7, 8, 9, 63, 64, 65, 77, 127, 128, 129, 136, 255, 256, 264, 511, 512, 513, 520, 768, 1000, 1023, 1024, 1025, 1536, 2047, 2048,
-           2049, 2056, 4095, 4096, 4104, 5000, 8191, 8192, 8193, 8200, 16001, 16384, 16385, 16392, 32768, 32776, 40000]
+LENGTHS = [1, 2, 7, 8, 9, 63, 64, 65, 77, 127, 128, 129, 136, 255, 256, 264, 511, 512, 513, 520, 768, 769, 776, 1000, 1023, 1024, 1025, 1280, 1536, 1537, 1544, 2047, 2048,
+           2049, 2056, 4095, 4096, 4104, 5000, 6143, 6144, 6145, 6152, 8191, 8192, 8193, 8200, 16001, 16384, 16385, 16392, 32768, 32776, 40000]
 
 
 @pytest.mark.parametrize("rms", [False, True], ids=["layer", "rms"])
@@ -165,7 +165,7 @@ def test_row_lengths(d, rms):
 
 
 @pytest.mark.parametrize("rms", [False, True], ids=["layer", "rms"])
-@pytest.mark.parametrize("d", [5, 77, 512, 768, 1030, 4096, 9000, 33000])
+@pytest.mark.parametrize("d", [5, 77, 512, 768, 1030, 1280, 1533, 4096, 5120, 6141, 9000, 33000])
 @pytest.mark.parametrize("x,w,r", [("f32", "f32", "f32"), ("bf16", "bf16", "bf16"), ("bf16", "f32", "f32"), ("f16", "f16", "f16"),
                                    ("f16", "f32", "f16"), ("bf16", "bf16", "f32"), ("f16", "", "f32"), ("bf16", "f32", "")])
 def test_fused_types(d, x, w, r, rms):
