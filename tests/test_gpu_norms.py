@@ -532,6 +532,36 @@ def test_captured_steps_replay():
             assert all(torch.equal(p, q) for p, q in zip(got, want)), k
 
 
+@pytest.mark.filterwarnings("ignore:The AccumulateGrad node's stream")
+@pytest.mark.parametrize("op", ["norm", "dropout"])
+def test_capture_beside_a_living_eager_graph_is_refused(op):
+    """The leaf's accumulation node is the eager graph's, on the default stream: refused in the capture, not outside it."""
+    w = torch.randn(96, device=dev(), requires_grad=True)
+    x = torch.randn(40, 96, device=dev(), requires_grad=True)
+
+    def step(dy):
+        y = F.rms_norm(x, w) if op == "norm" else F.dropout(x, 0.25, (3, 4))
+        return torch.autograd.grad(y, (x, w) if op == "norm" else x, dy)
+
+    dy = torch.randn(40, 96, device=dev())
+    want = step(dy)
+    alive = (x * w).sum()
+    with pytest.raises(RuntimeError, match="keep a graph of the same leaves alive"):
+        amd.GraphedStep(step, [dy])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                # another stream alone is no reason
+        got = step(dy)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    del alive
+    graphed = amd.GraphedStep(step, [dy])
+    for _ in range(3):
+        got = [t.clone() for t in graphed(dy)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_recomputed_forward_draws_the_same():
     # activation checkpointing runs the forward pass again under the generator state that it saved
     from torch.utils.checkpoint import checkpoint

@@ -7,6 +7,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -140,6 +141,25 @@ variable_list once(variable_list grads) {
     return (*error)(std::move(marked));
 }
 
+// A gradient that is captured into a graph must not go to a node on the default stream, which may not join a capture.  The engine would
+// have it wait there nonetheless and end the process.  A leaf's accumulation node belongs to the stream of the oldest graph
+// of it that still lives: an eager one, kept alive by a loss, puts it on the default stream.
+void refuse_default_stream(const char* what) {
+    const auto node = torch::autograd::get_current_node();
+    for (const torch::autograd::Edge& edge : node->next_edges()) {
+        if (!edge.function) continue;
+        const auto stream = edge.function->stream();
+        if (!stream || *stream != c10::Stream(c10::Stream::DEFAULT, stream->device())) continue;
+        const auto current = c10::hip::getCurrentHIPStream(stream->device_index());
+        if (current.id() == stream->id()) continue;
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(current.stream(), &capture) != hipSuccess) (void)hipGetLastError();
+        TORCH_CHECK(capture == hipStreamCaptureStatusNone, what, ": the captured backward pass leads to ", edge.function->name(),
+                    " on the default stream, which cannot be captured; release the eager results (a loss, an output) that keep "
+                    "a graph of the same leaves alive, then capture again");
+    }
+}
+
 // A node's inputs that may be missing go as optionals; the gradient edges are numbered over those that are there.
 using MaybeTensor = std::optional<Tensor>;
 MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
@@ -169,6 +189,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
         return dropout_launch(x, residual, p, rng, residual.defined() ? residual.scalar_type() : x.scalar_type());
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_default_stream("dropout");
         const Rng rng{ctx->get_saved_variables()[0], (uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["offset"].toInt()};
         Tensor dx;
         if (ctx->needs_input_grad(0)) {
@@ -239,6 +260,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_default_stream("norm");
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &residual = saved[1], &mean = saved[3], &rstd = saved[4];
         const auto meta = ctx->saved_data["meta"].toIntVector();
