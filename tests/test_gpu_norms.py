@@ -333,6 +333,21 @@ def test_large_offsets_keep_their_digits():
         close(y, want, bound, d)
 
 
+@pytest.mark.parametrize("start", [0, 1000])
+@pytest.mark.parametrize("d", [20000, 2000000])
+def test_long_rows_that_start_unlike_their_rest(d, start):
+    # the deviations are summed about a guess of the mean that the row's unlike part must not decide
+    g = torch.Generator(device=dev()).manual_seed(d)
+    x = torch.randn(3, d, generator=g, device=dev())
+    x[:, start:start + 2048] += 1000.0
+    y = F.layer_norm(x, eps=1e-6)
+    v = n64(x)
+    want, _, rstd = orc.norm_forward(v, None, None, 1e-6, False)
+    # a thread adds d / 256 terms; six standard deviations of that many roundings, on the value and on the mean
+    bound = H * (6 * np.sqrt(d / 256) + 8) * (np.abs(want) + rstd * np.abs(v - v.mean(1, keepdims=True)).mean(1, keepdims=True))
+    close(y, want, bound, d)
+
+
 def test_gradient_against_differences():
     g = torch.Generator(device=dev()).manual_seed(8)
     x, r = (torch.randn(12, 200, generator=g, device=dev()).requires_grad_(True) for _ in range(2))
