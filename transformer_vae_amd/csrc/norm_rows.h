@@ -620,7 +620,7 @@ __global__ __launch_bounds__(256) void norm_fwd_wide_kernel(NormCall c) {
             // a first guess of the mean from 2048 elements at 32 places of the row (these rows are longer): it is off by at most
             // sqrt(d / 2048) standard deviations, and by next to nothing for most rows, so sums about it lose nothing and the row
             // is read twice, not three times.  Not from the row's start alone: 2000000 elements, the first 2048 a thousand above
-            // the others' unit spread: 6e-3 off there, 5e-6 with this.
+            // the others' unit spread: 6e-3 off there, 6e-6 with this.
             float v[8];
             value8<T, R>(c, ph, row, (int)((long long)(threadIdx.x >> 3) * c.groups / 32) + (threadIdx.x & 7), v);
             mu = block_sum(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])), sm) * (1.f / 2048.f);
