@@ -6,7 +6,14 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
 import transformer_vae_amd as amd
+from transformer_vae_amd import _lib
 from transformer_vae_amd import functional as F
+
+
+@pytest.fixture(scope="module", autouse=True)
+def operators():
+    _lib.host()
+
 
 CALLS = [
     (lambda x, w: F.layer_norm(x, w, w), "norm", 1),
@@ -80,3 +87,28 @@ def test_recorded_operators_check_their_arguments():
                 call()
     with pytest.raises(NotImplementedError):        # no kernel for tensors of the CPU
         ops.dropout(torch.empty(4, 16), None, 0.1, None, 0, 0)
+
+
+@pytest.mark.parametrize("place", range(4))
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode_derivatives_are_refused(place, needs_grad):
+    """A tangent on any input, in any grad mode: never a result without one."""
+    import torch.autograd.forward_ad as fw
+    with FakeTensorMode(), fw.dual_level():
+        t = [torch.empty(s, device="cuda", requires_grad=needs_grad) for s in ((4, 16), (4, 16), (16,), (16,))]
+        t[place] = fw.make_dual(t[place], torch.empty_like(t[place]))
+        x, r, w, b = t
+        calls = [lambda: F.dropout_add_layer_norm(x, r, w, b, 1e-5, 0.1, (1, 2), True)]
+        if place != 1:
+            calls.append(lambda: F.layer_norm(x, w, b))
+        if place != 3:
+            calls.append(lambda: F.dropout_add_rms_norm(x, r, w))
+        if place < 2:
+            calls.append(lambda: F.dropout_add(x, r, 0.1, (1, 2)))
+        if place == 0:
+            calls += [lambda: F.dropout(x, 0.1), lambda: F.rms_norm(x)]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

@@ -8,6 +8,7 @@
 // make_fx, fake tensors -- sees one operator where a kernel launched beside the dispatcher would leave nothing but the
 // allocation of its output.  Their kernels check everything they are given, since a recorded graph calls them directly.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -182,6 +183,12 @@ void refuse_default_stream(const char* what) {
 MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
 Tensor tensor_of(const MaybeTensor& t) { return t ? *t : Tensor(); }
 bool wants_gradient(const MaybeTensor& t) { return t && t->requires_grad(); }
+// there is no forward-mode derivative: an input that carries a tangent is refused, whether it requires a gradient or not
+void refuse_tangents(const char* what, std::initializer_list<const MaybeTensor*> inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const MaybeTensor* t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!*t || !(*t)->_fw_grad(0).defined(), what, ": forward-mode derivatives are not implemented");
+}
 template <typename Signature>
 auto operator_handle(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
@@ -238,6 +245,8 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
 };
 
 Tensor dropout_autograd(const Tensor& x, const MaybeTensor& residual, double p, const MaybeTensor& rng, int64_t seed, int64_t offset, MaybeType type) {
+    const MaybeTensor input(x);
+    refuse_tangents("dropout", {&input, &residual});
     if (!type && at::GradMode::is_enabled() && (x.requires_grad() || wants_gradient(residual)))
         return DropoutNode::apply(x, residual, p, rng, seed, offset);
     const at::AutoDispatchBelowADInplaceOrView below;
@@ -422,6 +431,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
 
 std::vector<Tensor> norm_autograd(const Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight, const MaybeTensor& bias, int64_t kind,
                                   double eps, double p, const MaybeTensor& rng, int64_t seed, int64_t offset, bool return_sum, bool stats) {
+    const MaybeTensor input(x);
+    refuse_tangents("norm", {&input, &residual, &weight, &bias});
     if (!stats && at::GradMode::is_enabled() && (x.requires_grad() || wants_gradient(residual) || wants_gradient(weight) || wants_gradient(bias)))
         return NormNode::apply(x, residual, weight, bias, kind, eps, p, rng, seed, offset, return_sum);
     const at::AutoDispatchBelowADInplaceOrView below;
