@@ -124,13 +124,24 @@ class LatentDecoderT5Norm(LatentDecoderNTokens):
         self.norm = T5LayerFF(t_config)
         t_config.dropout_rate = dropout_rate
 
+    def _normed(self, h):
+        """The block's norm of ``h`` in the type that the stock one hands to the products: a 16-bit weight's, else the wider of the
+        two.  Under autocast the products round to its type themselves, so a norm of such an ``h`` may return it at once."""
+        weight, eps = self.norm.layer_norm.weight, self.norm.layer_norm.variance_epsilon
+        dtype = weight.dtype if weight.dtype in (torch.bfloat16, torch.float16) else torch.promote_types(h.dtype, weight.dtype)
+        if torch.is_autocast_enabled() and h.dtype == torch.get_autocast_dtype("cuda"):
+            dtype = h.dtype
+        if h.dtype != dtype:
+            h = h.float()
+        if weight.dtype != h.dtype:
+            weight = weight.float()
+        return F.rms_norm(h, weight, eps).to(dtype)
+
     def forward(self, latent) -> torch.Tensor:
         h = self._decode(latent)
         if not self.native_norm:
             return self.norm(h)
-        ln = self.norm.layer_norm
-        weight = ln.weight if ln.weight.dtype in (h.dtype, torch.float32) else ln.weight.float()
-        branch = self.norm.DenseReluDense(F.rms_norm(h, weight, ln.variance_epsilon))
+        branch = self.norm.DenseReluDense(self._normed(h))
         return F.dropout_add(branch, h if h.dtype == branch.dtype else h.float(), self._active_dropout())
 
 
