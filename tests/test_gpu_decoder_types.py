@@ -65,3 +65,29 @@ def test_t5_decoder_of_mixed_types_with_a_dropout_rate(z_type, p_type):
     assert a.dtype == c.dtype and (a.double() - c.double()).norm() <= 32 * max(u_of(z_type), u_of(p_type)) * a.double().norm()
     out = drop.train()(z)
     assert out.dtype == a.dtype and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("key", ["", "no_norm", "t5_norm"])
+@pytest.mark.parametrize("L", [24, 64])
+def test_double_latents_with_a_dropout_rate(key, L):
+    """The latent decoders compute float64 in fp32 and return float64; a dropout rate changes nothing about that."""
+    cfg = t5_cfg(L)
+    cfg.funnel = SimpleNamespace(d_model=64, layer_norm_eps=1e-9)
+    torch.manual_seed(4)
+    dec = amd.VAE_DECODER_MODELS[key](cfg, dropout_rate=0.25).to(dev(), F64)
+    z = torch.randn(4, 3, L, device=dev(), dtype=F64, requires_grad=True)
+    dec.train()
+    torch.manual_seed(9)
+    out = dec(z)
+    assert out.dtype == F64
+    grads = torch.autograd.grad(out.square().sum(), [z, *dec.parameters()])
+    assert all(g.dtype == F64 and torch.isfinite(g).all() for g in grads)
+    single = amd.VAE_DECODER_MODELS[key](cfg, dropout_rate=0.25).to(dev())
+    single.load_state_dict(dec.state_dict())
+    single.train()
+    torch.manual_seed(9)
+    want = single(z.detach().float())
+    # the same keep decisions; the stock products of t5_norm run in fp64 there and in fp32 here: 64 and 160 terms, twice 1.6 * 2.6
+    # of their rounding and a rounding a step, within 64 of fp32's in the 2-norm
+    assert (out.detach() - want.detach().double()).norm() <= 64 * u_of(F32) * out.detach().norm()
+    assert dec.eval()(z).dtype == F64

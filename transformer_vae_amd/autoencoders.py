@@ -49,6 +49,11 @@ class LatentEncoderNTokens(nn.Module):
 LatentEncoderLargeTanh = LatentEncoderNTokens
 
 
+def _single(t: torch.Tensor) -> torch.Tensor:
+    """float64 as fp32, in which the latent decoders compute it."""
+    return t.float() if t.dtype == torch.float64 else t
+
+
 class LatentDecoderNTokens(nn.Module):
     """Latent tokens -> full token hidden states (autoencoders.py:25-39).
 
@@ -84,7 +89,7 @@ class LatentDecoderNTokens(nn.Module):
 
     def forward(self, latent) -> torch.Tensor:
         out, p = self._decode(latent), self._active_dropout()
-        return F.dropout(out, p) if p > 0.0 else out
+        return F.dropout(_single(out), p).to(out.dtype) if p > 0.0 else out
 
 
 class LatentDecoderFunnelNorm(LatentDecoderNTokens):
@@ -98,9 +103,10 @@ class LatentDecoderFunnelNorm(LatentDecoderNTokens):
         w, b = self._linear_params()
         p = self._active_dropout()
         if p > 0.0:                # LayerNorm(dropout(linear)), as the Funnel's own sub-layers order them
-            r = self._decode(latent)
+            out = self._decode(latent)
+            r = _single(out)
             g, c = (t if t.dtype in (r.dtype, torch.float32) else t.float() for t in (self.norm.weight, self.norm.bias))
-            return F.dropout_add_layer_norm(r, None, g, c, self.norm.eps, p)
+            return F.dropout_add_layer_norm(r, None, g, c, self.norm.eps, p).to(out.dtype)
         return F.latent_decode(latent, w, b, self.norm.weight, self.norm.bias, self.norm.eps)
 
 
@@ -131,7 +137,7 @@ class LatentDecoderT5Norm(LatentDecoderNTokens):
         dtype = weight.dtype if weight.dtype in (torch.bfloat16, torch.float16) else torch.promote_types(h.dtype, weight.dtype)
         if torch.is_autocast_enabled() and h.dtype == torch.get_autocast_dtype("cuda"):
             dtype = h.dtype
-        if h.dtype != dtype:
+        if h.dtype != dtype or dtype == torch.float64:
             h = h.float()
         if weight.dtype != h.dtype:
             weight = weight.float()
@@ -142,7 +148,9 @@ class LatentDecoderT5Norm(LatentDecoderNTokens):
         if not self.native_norm:
             return self.norm(h)
         branch = self.norm.DenseReluDense(self._normed(h))
-        return F.dropout_add(branch, h if h.dtype == branch.dtype else h.float(), self._active_dropout())
+        x, r = _single(branch), _single(h)
+        out = F.dropout_add(x, r if r.dtype == x.dtype else r.float(), self._active_dropout())
+        return out.to(torch.promote_types(h.dtype, branch.dtype))
 
 
 # alias for the name used in the north-star description
