@@ -31,7 +31,8 @@ int norm_launch_f16(const NormCall& c, int r_dtype, bool bwd, hipStream_t s);
 namespace {
 
 // sum over the 256 threads of a workgroup, the same bits in every thread
-__device__ __forceinline__ float block_sum(float v, float* sm) {
+template <typename V>
+__device__ __forceinline__ V block_sum(V v, V* sm) {
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
@@ -610,12 +611,20 @@ __global__ __launch_bounds__(256) void norm_bwd_small_kernel(NormCall c, int row
 }
 
 // ---- longer rows: one workgroup per row, the row is read again for every pass over it ----------------------------
+// Eight neighbours are added in fp32, all further ones in fp64: a thread adds d / 2048 of them one after another, where fp32 would
+// lose up to as many roundings (2000000 equal values: their RMS norm was 2.2e-5 of itself off).  Two fp64 additions for eight
+// elements cost nothing beside the loads (2048 x 40000 bf16 forward 116 us either way, with its backward pass 364).
+__device__ __forceinline__ float sum8(const float v[8]) { return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])); }
+__device__ __forceinline__ float dot8(const float a[8], const float b[8]) {
+    return (fmaf(a[1], b[1], a[0] * b[0]) + fmaf(a[3], b[3], a[2] * b[2])) + (fmaf(a[5], b[5], a[4] * b[4]) + fmaf(a[7], b[7], a[6] * b[6]));
+}
+
 template <typename T, typename R>
 __global__ __launch_bounds__(256) void norm_fwd_wide_kernel(NormCall c) {
-    __shared__ float sm[4];
+    __shared__ double sm[4];
     const Philox ph(c.drop);
     for (long long row = blockIdx.x; row < c.rows; row += gridDim.x) {
-        float mu = 0.f, m2 = 0.f, q = 0.f;
+        float mu = 0.f, m2 = 0.f;
         if (!c.rms) {
             // a first guess of the mean from 2048 elements at 32 places of the row (these rows are longer): it is off by at most
             // sqrt(d / 2048) standard deviations, and by next to nothing for most rows, so sums about it lose nothing and the row
@@ -623,26 +632,25 @@ __global__ __launch_bounds__(256) void norm_fwd_wide_kernel(NormCall c) {
             // the others' unit spread: 6e-3 off there, 6e-6 with this.
             float v[8];
             value8<T, R>(c, ph, row, (int)((long long)(threadIdx.x >> 3) * c.groups / 32) + (threadIdx.x & 7), v);
-            mu = block_sum(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])), sm) * (1.f / 2048.f);
+            mu = (float)block_sum((double)sum8(v), sm) * (1.f / 2048.f);
         }
-        float t1 = 0.f;
+        double t1 = 0.0, q = 0.0;
         for (int g = threadIdx.x; g < c.groups; g += 256) {
             float v[8];
             value8<T, R>(c, ph, row, g, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float t = 8 * g + e < c.d ? v[e] - mu : 0.f;
-                t1 += t;
-                q = fmaf(t, t, q);
-            }
+            for (int e = 0; e < 8; ++e) v[e] = 8 * g + e < c.d ? v[e] - mu : 0.f;
+            t1 += (double)sum8(v);
+            q += (double)dot8(v, v);
         }
-        q = block_sum(q, sm) / (float)c.d;
+        q = block_sum(q, sm) / (double)c.d;
         if (!c.rms) {
-            m2 = block_sum(t1, sm) / (float)c.d;
-            q -= m2 * m2;
-            if (q < 0.f) q = 0.f;
+            t1 = block_sum(t1, sm) / (double)c.d;
+            q -= t1 * t1;
+            if (q < 0.0) q = 0.0;
+            m2 = (float)t1;
         }
-        const float rs = rsqrtf(q + c.eps);
+        const float rs = rsqrtf((float)q + c.eps);
         for (int g = threadIdx.x; g < c.groups; g += 256) {
             float v[8], w[8], b[8];
             const int nv = c.d - 8 * g;
@@ -663,12 +671,12 @@ __global__ __launch_bounds__(256) void norm_fwd_wide_kernel(NormCall c) {
 
 template <typename T, typename R>
 __global__ __launch_bounds__(256) void norm_bwd_wide_kernel(NormCall c) {
-    __shared__ float sm[4];
+    __shared__ double sm[4];
     const Philox ph(c.drop);
     for (long long row = blockIdx.x; row < c.rows; row += gridDim.x) {
         const float mu = c.mean ? c.mean[row] : 0.f, rs = c.rstd[row];
         const T* dy = static_cast<const T*>(c.dy) + row_offset(c.dy_rows, c.grp, row);
-        float s1 = 0.f, s2 = 0.f;
+        double t1 = 0.0, t2 = 0.0;
         for (int g = threadIdx.x; g < c.groups; g += 256) {
             float v[8], w[8], u[8];
             const int nv = c.d - 8 * g;
@@ -677,13 +685,14 @@ __global__ __launch_bounds__(256) void norm_bwd_wide_kernel(NormCall c) {
             load8_param<T>(c.weight, c.w_f32, 8 * g, nv, 1.f, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float gw = u[e] * w[e];
-                s1 += gw;
-                s2 = fmaf(gw, (v[e] - mu) * rs, s2);
+                u[e] *= w[e];
+                v[e] = (v[e] - mu) * rs;
             }
+            t1 += (double)sum8(u);
+            t2 += (double)dot8(u, v);
         }
-        s2 = block_sum(s2, sm) / (float)c.d;
-        s1 = c.rms ? 0.f : block_sum(s1, sm) / (float)c.d;
+        const float s2 = (float)(block_sum(t2, sm) / (double)c.d);
+        const float s1 = c.rms ? 0.f : (float)(block_sum(t1, sm) / (double)c.d);
         for (int g = threadIdx.x; g < c.groups; g += 256) {
             float v[8], w[8], u[8];
             const int nv = c.d - 8 * g;
