@@ -45,3 +45,23 @@ def test_equal_gradients_add_up(d, rms):
     bound = H * rstd * (32 * 0.7 + 24 * 0.7 * np.abs(xh) * np.abs(xh).mean(1, keepdims=True) + 16 * np.abs(xh) * np.abs((0.7 * xh).mean(1, keepdims=True)))
     off = np.abs(n64(dx) - want)
     assert (off <= bound).all(), (off.max(), (off / bound).max())
+
+
+@pytest.mark.parametrize("unlike", [64, 1])
+@pytest.mark.parametrize("parts", [32, 64, 7])
+@pytest.mark.parametrize("d", [20000, 200000, 2000000])
+def test_rows_of_segments_that_start_unlike_their_rest(d, parts, unlike):
+    """Concatenated blocks with a header: whatever places the first guess of the mean comes from, it must not decide the result."""
+    g = torch.Generator(device=dev()).manual_seed(d + parts)
+    x = torch.randn(3, d, generator=g, device=dev())
+    for k in range(parts):
+        at = (k * ((d + 7) // 8) // parts) * 8                # where a segment of whole groups of eight starts
+        x[:, at:at + unlike] += 1000.0
+    y = F.layer_norm(x, eps=1e-6)
+    v = n64(x)
+    want, _, rstd = orc.norm_forward(v, None, None, 1e-6, False)
+    # a difference to the mean costs 2 h of itself (mean and remainder), the statistics and the products 16 h of the value; the mean
+    # is off by 2 h of the first guess's remaining distance, a standard deviation at most, and of itself
+    bound = H * (20 * np.abs(want) + 4 + 2 * rstd * np.abs(v.mean(1, keepdims=True)))
+    off = np.abs(n64(y) - want)
+    assert (off <= bound).all(), (off.max(), (off / bound).max())

@@ -626,30 +626,39 @@ __global__ __launch_bounds__(256) void norm_fwd_wide_kernel(NormCall c) {
     for (long long row = blockIdx.x; row < c.rows; row += gridDim.x) {
         float mu = 0.f, m2 = 0.f;
         if (!c.rms) {
-            // a first guess of the mean from 2048 elements at 32 places of the row (these rows are longer): it is off by at most
-            // sqrt(d / 2048) standard deviations, and by next to nothing for most rows, so sums about it lose nothing and the row
-            // is read twice, not three times.  Not from the row's start alone: 2000000 elements, the first 2048 a thousand above
-            // the others' unit spread: 6e-3 off there, 6e-6 with this.
+            // A first guess of the mean from 2048 elements at 32 places of the row (these rows are longer).  It is off by next to
+            // nothing for most rows, so sums about it lose nothing and the row is read twice, not three times.
             float v[8];
             value8<T, R>(c, ph, row, (int)((long long)(threadIdx.x >> 3) * c.groups / 32) + (threadIdx.x & 7), v);
             mu = (float)block_sum((double)sum8(v), sm) * (1.f / 2048.f);
         }
         double t1 = 0.0, q = 0.0;
-        for (int g = threadIdx.x; g < c.groups; g += 256) {
-            float v[8];
-            value8<T, R>(c, ph, row, g, v);
+        const auto sums = [&] {
+            t1 = q = 0.0;
+            for (int g = threadIdx.x; g < c.groups; g += 256) {
+                float v[8];
+                value8<T, R>(c, ph, row, g, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 8 * g + e < c.d ? v[e] - mu : 0.f;
-            t1 += (double)sum8(v);
-            q += (double)dot8(v, v);
-        }
-        q = block_sum(q, sm) / (double)c.d;
-        if (!c.rms) {
+                for (int e = 0; e < 8; ++e) v[e] = 8 * g + e < c.d ? v[e] - mu : 0.f;
+                t1 += (double)sum8(v);
+                q += (double)dot8(v, v);
+            }
+            q = block_sum(q, sm) / (double)c.d;
+            if (c.rms) return;
             t1 = block_sum(t1, sm) / (double)c.d;
             q -= t1 * t1;
             if (q < 0.0) q = 0.0;
-            m2 = (float)t1;
+        };
+        sums();
+        // Where those places are unlike the rest the guess can be off by sqrt(d / 2048) standard deviations, and every difference to
+        // it carries a rounding of that much.  Beyond one standard deviation the sums are taken again, about the mean that they
+        // gave (2000000 elements, the first 64 of each 32nd a thousand above the others' unit spread: half of the results
+        // were over 4e-5 of themselves off, 5e-8 now).  All threads have the same sums.
+        if (!c.rms && t1 * t1 > q) {
+            mu += (float)t1;
+            sums();
         }
+        if (!c.rms) m2 = (float)t1;
         const float rs = rsqrtf((float)q + c.eps);
         for (int g = threadIdx.x; g < c.groups; g += 256) {
             float v[8], w[8], b[8];
