@@ -627,7 +627,8 @@ def _slerp(t1, t2, ratio):
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """Layer norm over the last axis of ``x`` (float32, bfloat16 or float16), differentiable once.  ``weight`` and ``bias`` are
     of x's type or float32 (mixed precision) and may be missing; the result is of x's type, statistics and sums are fp32.
-    Rows of any strides along up to two leading axes are read where they lie."""
+    Rows of any strides along up to two leading axes are read where they lie.  The same call repeats bit for bit; x's gradient
+    alone and beside the weights' can come from different kernels (up to 512 rows of 2048) and then agrees to fp32's rounding."""
     return _lib.host().norm("layer_norm", _lib.TVAE_NORM_LAYER, x, None, weight, bias, eps, 0.0, None, False)
 
 
