@@ -90,7 +90,7 @@ def build(force: bool = False) -> str:
     """Compile csrc/*.hip into libtvae_hip.so for gfx950 and csrc/host.cpp into _host.so.  Works without a GPU."""
     if force:
         subprocess.run(["make", "-C", CSRC, "clean"], check=True, capture_output=True)
-    proc = subprocess.run(["make", "-C", CSRC, "-j4"], capture_output=True, text=True)
+    proc = subprocess.run(["make", "-C", CSRC, "-j4", "all", "host"], capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("building libtvae_hip.so failed:\n" + proc.stdout + proc.stderr)
     return LIB_PATH
@@ -123,7 +123,7 @@ def host():
         lib()
         if not os.path.exists(HOST_PATH):
             raise RuntimeError(f"{HOST_PATH} is missing: the extension has not been built "
-                               "(run `python -c 'import __graft_entry__ as g; g.build()'` or `make -C transformer_vae_amd/csrc`). "
+                               "(run `python -c 'import __graft_entry__ as g; g.build()'` or `make -C transformer_vae_amd/csrc all host`). "
                                "There is no CPU fallback for this path.")
         from . import _host as module
         _host = module
