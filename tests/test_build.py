@@ -21,3 +21,19 @@ def test_the_library_is_built_without_torch():
     assert "libtvae_hip.so" in plan and "host.cpp" not in plan and "python" not in plan
     plan = planned("all", "host")
     assert "libtvae_hip.so" in plan and "host.cpp" in plan
+
+
+def test_the_nodes_call_the_library_that_was_loaded(tmp_path):
+    """Where another build of the library is put in the default's place, the autograd nodes follow, and no second copy is mapped."""
+    other = tmp_path / "libtvae_other.so"
+    other.write_bytes(open(_lib.LIB_PATH, "rb").read())
+    code = (f"from transformer_vae_amd import _lib; _lib.LIB_PATH = {str(other)!r}; _lib.host(); "
+            "print({l.split()[-1] for l in open('/proc/self/maps') if 'libtvae' in l})")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, check=True, cwd=ROOT).stdout
+    assert eval(out) == {str(other)}
+
+
+def test_a_library_without_the_operators_is_named():
+    code = ("import ctypes; from transformer_vae_amd import _lib; h = _lib.host(); "
+            "import pytest\nwith pytest.raises(RuntimeError, match='tvae_last_error'): h.bind(ctypes.CDLL('libc.so.6')._handle)")
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)

@@ -120,12 +120,12 @@ def host():
     """The module of C++ autograd nodes (loads on first use; raises if it has not been built)."""
     global _host
     if _host is None:
-        lib()
         if not os.path.exists(HOST_PATH):
             raise RuntimeError(f"{HOST_PATH} is missing: the extension has not been built "
                                "(run `python -c 'import __graft_entry__ as g; g.build()'` or `make -C transformer_vae_amd/csrc all host`). "
                                "There is no CPU fallback for this path.")
         from . import _host as module
+        module.bind(lib()._handle)
         _host = module
     return _host
 

@@ -18,6 +18,8 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
+#include <dlfcn.h>
+
 #include <array>
 #include <cstdint>
 #include <optional>
@@ -36,8 +38,36 @@ using torch::autograd::variable_list;
 using MaybeTensor = std::optional<Tensor>;
 using MaybeType = std::optional<at::ScalarType>;
 
+// The library's entry points, of the one that the package has loaded: this module is not linked to it, so that there is one copy,
+// whichever build of it that is.
+struct Library {
+    decltype(&tvae_last_error) last_error = nullptr;
+    decltype(&tvae_dropout) dropout = nullptr;
+    decltype(&tvae_norm_fwd) norm_fwd = nullptr;
+    decltype(&tvae_norm_bwd) norm_bwd = nullptr;
+    decltype(&tvae_norm_bwd_workspace_bytes) norm_bwd_workspace_bytes = nullptr;
+} bound;
+void bind(uintptr_t handle) {
+    const auto find = [&](auto& entry, const char* name) {
+        void* const at = dlsym(reinterpret_cast<void*>(handle), name);
+        TORCH_CHECK(at, "the library has no ", name, ": it was not built from these sources");
+        entry = reinterpret_cast<std::decay_t<decltype(entry)>>(at);
+    };
+    Library l;
+    find(l.last_error, "tvae_last_error");
+    find(l.dropout, "tvae_dropout");
+    find(l.norm_fwd, "tvae_norm_fwd");
+    find(l.norm_bwd, "tvae_norm_bwd");
+    find(l.norm_bwd_workspace_bytes, "tvae_norm_bwd_workspace_bytes");
+    bound = l;
+}
+const Library& library() {
+    TORCH_CHECK(bound.dropout, "the operators' library has not been loaded (transformer_vae_amd loads it with the first call)");
+    return bound;
+}
+
 void check(int status, const char* what) {
-    TORCH_CHECK(status == 0, what, " failed (status ", status, "): ", tvae_last_error());
+    TORCH_CHECK(status == 0, what, " failed (status ", status, "): ", library().last_error());
 }
 
 int code_of(at::ScalarType t) {
@@ -209,7 +239,7 @@ Tensor dropout_cuda(const Tensor& x, const MaybeTensor& residual_, double p, con
     const Tensor out = dropout_out(x, residual_, p, rng, seed, offset, type);
     const Rows l(x.sizes(), {x, residual});
     if (l.rows * l.d > 0)
-        check(tvae_dropout(ptr(l.r[0].t), l.r[0].so, l.r[0].si, ptr(l.r[1].t), l.r[1].so, l.r[1].si, l.grp, out_ptr(out), l.rows, l.d, p,
+        check(library().dropout(ptr(l.r[0].t), l.r[0].so, l.r[0].si, ptr(l.r[1].t), l.r[1].so, l.r[1].si, l.grp, out_ptr(out), l.rows, l.d, p,
                            rng_ptr(rng), (uint64_t)seed, (uint64_t)offset, code_of(x.scalar_type()), code_of(out.scalar_type()),
                            stream_of(x)), "tvae_dropout");
     return out;
@@ -298,7 +328,7 @@ std::vector<Tensor> norm_cuda(const Tensor& x, const MaybeTensor& residual_, con
     const at::ScalarType w_type = weight.defined() ? weight.scalar_type() : bias.defined() ? bias.scalar_type() : x.scalar_type();
     const size_t at_rstd = return_sum ? 2 : 1;
     if (l.rows > 0)
-        check(tvae_norm_fwd((int)kind, ptr(l.r[0].t), l.r[0].so, l.r[0].si, ptr(l.r[1].t), l.r[1].so, l.r[1].si, l.grp, ptr(weight), ptr(bias), eps,
+        check(library().norm_fwd((int)kind, ptr(l.r[0].t), l.r[0].so, l.r[0].si, ptr(l.r[1].t), l.r[1].so, l.r[1].si, l.grp, ptr(weight), ptr(bias), eps,
                             p, rng_ptr(rng), (uint64_t)seed, (uint64_t)offset, out_ptr(out[0]), return_sum ? out_ptr(out[1]) : nullptr,
                             stats && kind != TVAE_NORM_RMS ? (float*)out_ptr(out[at_rstd + 1]) : nullptr,
                             stats ? (float*)out_ptr(out[at_rstd]) : nullptr, l.rows, l.d, code_of(x.scalar_type()), code_of(w_type),
@@ -354,11 +384,11 @@ std::vector<Tensor> norm_backward_cuda(const Tensor& dy, const MaybeTensor& dsum
         return out;
     }
     Tensor ws;
-    const int64_t bytes = need[2] || need[3] ? tvae_norm_bwd_workspace_bytes(l.rows, l.d) : 0;
+    const int64_t bytes = need[2] || need[3] ? library().norm_bwd_workspace_bytes(l.rows, l.d) : 0;
     if (bytes > 0) ws = at::empty({bytes}, dy.options().dtype(at::kByte));
     const Tensor weight = weight_ ? weight_->contiguous() : Tensor();
     const at::ScalarType r_type = residual ? residual->scalar_type() : dy.scalar_type();
-    check(tvae_norm_bwd((int)kind, ptr(l.r[0].t), l.r[0].so, l.r[0].si, ptr(l.r[1].t), l.r[1].so, l.r[1].si, ptr(l.r[2].t), l.r[2].so, l.r[2].si,
+    check(library().norm_bwd((int)kind, ptr(l.r[0].t), l.r[0].so, l.r[0].si, ptr(l.r[1].t), l.r[1].so, l.r[1].si, ptr(l.r[2].t), l.r[2].so, l.r[2].si,
                         ptr(l.r[3].t), l.r[3].so, l.r[3].si, l.grp, ptr(weight), mean ? (const float*)ptr(*mean) : nullptr,
                         (const float*)ptr(rstd), p, rng_ptr(rng), (uint64_t)seed, (uint64_t)offset, out_ptr(grads[0]), out_ptr(grads[1]),
                         out_ptr(grads[2]), out_ptr(grads[3]), l.rows, l.d, code_of(dy.scalar_type()), code_of(w_type), code_of(r_type),
@@ -480,4 +510,5 @@ PYBIND11_MODULE(_host, m) {
     m.doc() = "autograd nodes of the norm and dropout operators";
     m.def("norm", &norm);
     m.def("dropout", &dropout);
+    m.def("bind", &bind);
 }
