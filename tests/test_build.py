@@ -37,3 +37,27 @@ def test_a_library_without_the_operators_is_named():
     code = ("import ctypes; from transformer_vae_amd import _lib; h = _lib.host(); "
             "import pytest\nwith pytest.raises(RuntimeError, match='tvae_last_error'): h.bind(ctypes.CDLL('libc.so.6')._handle)")
     subprocess.run([sys.executable, "-c", code], check=True, cwd=ROOT)
+
+
+def test_the_nodes_follow_torch(tmp_path):
+    """Built again where torch or Python have changed since, with the C++ ABI that torch was built with."""
+    import torch
+    pkg = tmp_path / "transformer_vae_amd"
+    for d in (pkg / "csrc", tmp_path / "include"):
+        d.mkdir(parents=True)
+    for f in ("Makefile", "host.cpp"):
+        (pkg / "csrc" / f).write_bytes(open(os.path.join(_lib.CSRC, f), "rb").read())
+    (tmp_path / "include" / "tvae_hip.h").write_bytes(open(_lib.HEADER, "rb").read())
+    (tmp_path / "bin").mkdir()
+    cxx = tmp_path / "bin" / "cxx"
+    cxx.write_text('#!/bin/sh\necho "$@" >> ' + str(tmp_path / "ran") + '\nwhile [ "$1" != -o ]; do shift; done\n: > "$2"\n')
+    cxx.chmod(0o755)
+    make = lambda: subprocess.run(["make", "-C", str(pkg / "csrc"), "host", f"CXX={cxx}", f"PYTHON={sys.executable}"], check=True, capture_output=True)
+    runs = lambda: (tmp_path / "ran").read_text().splitlines()
+    make(), make()
+    assert len(runs()) == 1
+    assert f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}" in runs()[0]
+    (stamp,) = [p for p in (pkg / "csrc").iterdir() if torch.__version__ in p.read_text(errors="replace")]
+    stamp.write_text(stamp.read_text().replace(torch.__version__, "1.0"))
+    make(), make()
+    assert len(runs()) == 2

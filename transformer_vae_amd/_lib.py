@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+import sys
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -90,7 +91,7 @@ def build(force: bool = False) -> str:
     """Compile csrc/*.hip into libtvae_hip.so for gfx950 and csrc/host.cpp into _host.so.  Works without a GPU."""
     if force:
         subprocess.run(["make", "-C", CSRC, "clean"], check=True, capture_output=True)
-    proc = subprocess.run(["make", "-C", CSRC, "-j4", "all", "host"], capture_output=True, text=True)
+    proc = subprocess.run(["make", "-C", CSRC, "-j4", "all", "host", f"PYTHON={sys.executable}"], capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("building libtvae_hip.so failed:\n" + proc.stdout + proc.stderr)
     return LIB_PATH
