@@ -61,3 +61,13 @@ def test_the_nodes_follow_torch(tmp_path):
     stamp.write_text(stamp.read_text().replace(torch.__version__, "1.0"))
     make(), make()
     assert len(runs()) == 2
+
+
+def test_other_flags_build_everything_again():
+    # objects of a tree from before a flag was set must not stay (that no packed fp32 instructions are used is one of them)
+    plan = subprocess.run(["make", "-n", "-W", "Makefile", "-C", _lib.CSRC], capture_output=True, text=True, check=True).stdout
+    sources = [f for f in os.listdir(_lib.CSRC) if f.endswith(".hip")]
+    lines = plan.splitlines()
+    for f in sources:
+        (line,) = [l for l in lines if f"-c {f}" in l]
+        assert "-packed-fp32-ops" in line
