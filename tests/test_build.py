@@ -71,3 +71,29 @@ def test_other_flags_build_everything_again():
     for f in sources:
         (line,) = [l for l in lines if f"-c {f}" in l]
         assert "-packed-fp32-ops" in line
+
+
+def test_variants_hold_every_source_built_as_the_library_is(tmp_path):
+    """tools/build_variant.sh: a variant that lacks a source lacks its entry points, and the package cannot load it."""
+    pkg = tmp_path / "transformer_vae_amd"
+    (pkg / "csrc").mkdir(parents=True)
+    (tmp_path / "tools").mkdir()
+    (tmp_path / "tools" / "build_variant.sh").write_bytes(open(os.path.join(ROOT, "tools", "build_variant.sh"), "rb").read())
+    sources = sorted(f[:-4] for f in os.listdir(_lib.CSRC) if f.endswith(".hip"))
+    (pkg / "csrc" / "Makefile").write_bytes(open(os.path.join(_lib.CSRC, "Makefile"), "rb").read())
+    for f in sources:
+        (pkg / "csrc" / (f + ".hip")).write_text("TVAE_SPLITS\n" if f == "mmd_q32" else "")
+        (pkg / "csrc" / (f + ".o")).write_text(f)
+    for f in ("tvae_common.h", "mmd_common.h", "mmd_q32.h", "norm_common.h", "norm_rows.h"):
+        (pkg / "csrc" / f).write_text("")
+    (tmp_path / "include").mkdir()
+    (tmp_path / "include" / "tvae_hip.h").write_text("")
+    hipcc = tmp_path / "hipcc"
+    hipcc.write_text('#!/bin/sh\necho "$@" >> ' + str(tmp_path / "ran") + '\nwhile [ "$1" != -o ]; do shift; done\necho variant > "$2"\n')
+    hipcc.chmod(0o755)
+    subprocess.run(["bash", str(tmp_path / "tools" / "build_variant.sh"), "x", "-DTVAE_SPLITS=3"], check=True, capture_output=True,
+                   env={**os.environ, "HIPCC": str(hipcc)})
+    compiled, linked = (tmp_path / "ran").read_text().splitlines()
+    assert "-c mmd_q32.hip" in compiled and "-DTVAE_SPLITS=3" in compiled and "-packed-fp32-ops" in compiled and "-fno-slp-vectorize" in compiled
+    assert {os.path.basename(w)[:-2] for w in linked.split() if w.endswith(".o")} == set(sources)
+    assert (pkg / "variants" / "libtvae_x.so").exists()
