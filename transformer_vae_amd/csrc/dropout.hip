@@ -21,7 +21,7 @@ struct DropoutCall {
     const void* in; const void* residual; void* out;
     RowsOf in_rows, res_rows;
     int grp, d, groups;                         // groups = ceil(d / 8)
-    long long rows;
+    long long rows, first;                      // first: the launch's first workgroup
     unsigned long long inv64; unsigned inv32;   // floor((2^64 - 1) / groups), floor((2^32 - 1) / groups)
     DropoutArgs drop;
 };
@@ -32,7 +32,7 @@ struct DropoutCall {
 template <typename A, typename O, bool NT, int GROUPS>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutCall c) {
     const Philox ph(c.drop);
-    const unsigned long long t0 = (unsigned long long)blockIdx.x * (256 * GROUPS);
+    const unsigned long long t0 = (unsigned long long)(c.first + blockIdx.x) * (256 * GROUPS);
     unsigned long long row0 = __umul64hi(t0, c.inv64);
     unsigned g0 = (unsigned)(t0 - row0 * (unsigned)c.groups);
     if (g0 >= (unsigned)c.groups) { ++row0; g0 -= (unsigned)c.groups; }
@@ -72,11 +72,15 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropoutCall c) {
 }
 
 template <typename A, typename O, bool NT, int GROUPS>
-int dropout_launch(const DropoutCall& c, hipStream_t s) {
+int dropout_launch(DropoutCall c, hipStream_t s) {
     const long long blocks = (c.rows * c.groups + 256 * GROUPS - 1) / (256 * GROUPS);
+    constexpr long long MOST = 1ll << 23;       // a launch has less than 2^32 threads
     TVAE_REQUIRE(blocks < (1ll << 31), "dropout: too many elements");
-    hipLaunchKernelGGL((dropout_kernel<A, O, NT, GROUPS>), dim3((unsigned)blocks), dim3(256), 0, s, c);
-    TVAE_CHECK_HIP(hipGetLastError());
+    for (c.first = 0; c.first < blocks; c.first += MOST) {
+        const long long left = blocks - c.first;
+        hipLaunchKernelGGL((dropout_kernel<A, O, NT, GROUPS>), dim3((unsigned)(left < MOST ? left : MOST)), dim3(256), 0, s, c);
+        TVAE_CHECK_HIP(hipGetLastError());
+    }
     return TVAE_OK;
 }
 // Long streams go past the caches.  Four groups a thread pay where they keep enough narrow loads in flight for that (bf16,
