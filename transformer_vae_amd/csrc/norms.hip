@@ -18,14 +18,14 @@ namespace {
 // dw, and db where blockIdx.y = 1 or there is no dw: the partial sums added in a fixed order, in fp64; COLS columns by
 // 1024 / COLS chunk lanes
 template <typename W, int COLS>
-__global__ __launch_bounds__(1024) void norm_param_final_kernel(const float* part, int chunks, int d, W* dw, W* db) {
+__global__ __launch_bounds__(1024) void norm_param_final_kernel(const float* part, int chunks, int d, int first, W* dw, W* db) {
     constexpr int LANES = 1024 / COLS, UNROLL = COLS == 64 ? 8 : 4;
     __shared__ double sm[LANES][COLS + 1];
     const bool second = blockIdx.y || !dw;
     W* out = second ? db : dw;
     const float* p = part + (second ? (long long)chunks * d : 0);
     const int cx = threadIdx.x % COLS, ry = threadIdx.x / COLS;
-    const long long col = (long long)blockIdx.x * COLS + cx;
+    const long long col = (long long)(first + blockIdx.x) * COLS + cx;
     double s = 0.0;
     if (col < d) {
 #pragma unroll UNROLL
@@ -50,15 +50,22 @@ int norm_dispatch(const NormCall& c, int dtype, int r_dtype, bool bwd, hipStream
     return dtype == TVAE_BF16 ? norm_launch_bf16(c, r_dtype, bwd, s) : norm_launch_f16(c, r_dtype, bwd, s);
 }
 
+template <typename W, int COLS>
+int norm_params_launch(const NormCall& c, hipStream_t s) {
+    W *dw = static_cast<W*>(c.dw), *db = static_cast<W*>(c.db);
+    const int blocks = (c.d + COLS - 1) / COLS;
+    constexpr int MOST = 1 << 21;               // a launch has less than 2^32 threads
+    for (int first = 0; first < blocks; first += MOST) {
+        const int n = blocks - first < MOST ? blocks - first : MOST;
+        hipLaunchKernelGGL((norm_param_final_kernel<W, COLS>), dim3((unsigned)n, dw && db ? 2 : 1), dim3(1024), 0, s, c.part, c.chunks, c.d, first, dw, db);
+        TVAE_CHECK_HIP(hipGetLastError());
+    }
+    return TVAE_OK;
+}
 // Long rows: 64 columns a workgroup, 256 bytes of every partial sum.  Short ones would leave most of the card idle then.
 template <typename W>
 int norm_params(const NormCall& c, hipStream_t s) {
-    W *dw = static_cast<W*>(c.dw), *db = static_cast<W*>(c.db);
-    const unsigned both = dw && db ? 2 : 1;
-    if (c.d >= 8192) hipLaunchKernelGGL((norm_param_final_kernel<W, 64>), dim3((unsigned)((c.d + 63) / 64), both), dim3(1024), 0, s, c.part, c.chunks, c.d, dw, db);
-    else hipLaunchKernelGGL((norm_param_final_kernel<W, 16>), dim3((unsigned)((c.d + 15) / 16), both), dim3(1024), 0, s, c.part, c.chunks, c.d, dw, db);
-    TVAE_CHECK_HIP(hipGetLastError());
-    return TVAE_OK;
+    return c.d >= 8192 ? norm_params_launch<W, 64>(c, s) : norm_params_launch<W, 16>(c, s);
 }
 
 // what both directions check and fill in
