@@ -112,3 +112,17 @@ def test_forward_mode_derivatives_are_refused(place, needs_grad):
                 call()
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_what_stands_for_a_dropout_state():
+    """A tensor, or two integers in any sequence; another thing is a TypeError, another number of them a ValueError."""
+    import numpy as np
+    with FakeTensorMode():
+        x = torch.empty(4, 16, device="cuda")
+        for rng in ((1, 2), [1, 2], np.array([1, 2]), (np.int64(1), True), (-1, 2 ** 64 - 1)):
+            assert F.dropout(x, 0.5, rng).shape == x.shape
+        for rng, error in ((7, TypeError), ("12", TypeError), (torch.Generator(), TypeError), ((1, 2.5), TypeError), (("1", "2"), TypeError), ({1, 2}, TypeError),
+                           ((1,), ValueError), ([1, 2, 3], ValueError), ((), ValueError)):
+            for call in (lambda: F.dropout(x, 0.5, rng), lambda: F.dropout_add_rms_norm(x, x, p=0.5, rng=rng)):
+                with pytest.raises(error, match="rng must be a tensor or two ints"):
+                    call()

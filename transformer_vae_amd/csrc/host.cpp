@@ -167,10 +167,15 @@ Rng rng_of(const char* what, const Tensor& x, double p, const pybind11::object& 
     } else if (THPVariable_Check(rng.ptr())) {
         r.state = THPVariable_Unpack(rng.ptr()).detach();
     } else {
-        const auto words = pybind11::cast<pybind11::tuple>(rng);
-        TORCH_CHECK_VALUE(words.size() == 2, what, ": rng is a tensor or two ints (seed, offset)");
-        const auto word = [](const pybind11::object& o) {
-            const uint64_t v = PyLong_AsUnsignedLongLongMask(pybind11::int_(o).ptr());
+        const bool sequence = PySequence_Check(rng.ptr()) && !PyUnicode_Check(rng.ptr()) && !PyBytes_Check(rng.ptr());
+        TORCH_CHECK_TYPE(sequence, what, ": rng must be a tensor or two ints (seed, offset), got ", Py_TYPE(rng.ptr())->tp_name);
+        const auto words = pybind11::reinterpret_borrow<pybind11::sequence>(rng);
+        TORCH_CHECK_VALUE(words.size() == 2, what, ": rng must be a tensor or two ints (seed, offset), got ", words.size(), " of them");
+        const auto word = [&](const pybind11::object& o) {
+            const auto index = pybind11::reinterpret_steal<pybind11::object>(PyNumber_Index(o.ptr()));
+            if (!index) PyErr_Clear();
+            TORCH_CHECK_TYPE(index, what, ": rng must be a tensor or two ints (seed, offset), got a ", Py_TYPE(o.ptr())->tp_name);
+            const uint64_t v = PyLong_AsUnsignedLongLongMask(index.ptr());
             if (PyErr_Occurred()) throw pybind11::error_already_set();
             return (int64_t)v;
         };
