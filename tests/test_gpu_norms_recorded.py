@@ -93,3 +93,37 @@ def test_traced_decoder():
         for batch in (2, 9):
             z = torch.randn(batch, 3, 64, generator=g, device=dev())
             assert torch.equal(traced(z), dec(z))
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_program_recorded_below_autograd_keeps_its_gradients(name):
+    """Recorded with inputs that require gradients, the graph holds the calls that stand below autograd; run as it is, it must not
+    give results without a history."""
+    call, dtype = CALLS[name], torch.bfloat16 if name == "pre_norm" else torch.float32
+
+    def leaves(seed):
+        new = inputs(40, 96, seed, dtype)
+        return [t.requires_grad_(True) for t in new[:4]] + list(new[4:])
+
+    graph = make_fx(lambda *t: call(*t))(*leaves(1))
+    new, grads = leaves(2), []
+    for f in (graph, call):
+        out = f(*new)
+        outs = out if isinstance(out, tuple) else (out,)
+        assert all(t.requires_grad for t in outs)
+        grads.append([g for g in torch.autograd.grad(outs, new[:4], [new[4]] * len(outs), allow_unused=True) if g is not None])
+    assert grads[0] and same(*grads)
+
+
+def test_a_recorded_backward_pass_is_not_differentiated():
+    def step(x, w, dy):
+        y = F.rms_norm(x, w)
+        return torch.autograd.grad(y, (x, w), dy)
+
+    x, r, w, b, dy, rng = inputs(40, 96, 1)
+    x.requires_grad_(True), w.requires_grad_(True)
+    graph = make_fx(step)(x, w, dy)
+    got = graph(x, w, dy)
+    assert same([t.detach() for t in got], step(x, w, dy))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        got[0].sum().backward()

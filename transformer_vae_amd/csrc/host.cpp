@@ -256,7 +256,7 @@ const auto& dropout_op() {
 
 struct DropoutNode : torch::autograd::Function<DropoutNode> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& residual, double p, const MaybeTensor& rng, int64_t seed,
-                          int64_t offset) {
+                          int64_t offset, MaybeType type) {
         ctx->saved_data["add"] = residual.has_value();
         ctx->save_for_backward({tensor_of(rng)});
         ctx->saved_data["p"] = p;
@@ -264,7 +264,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
         ctx->saved_data["offset"] = offset;
         ctx->saved_data["type"] = (int64_t)x.scalar_type();
         const at::AutoDispatchBelowADInplaceOrView below;
-        return dropout_op().call(x, residual, p, rng, seed, offset, std::nullopt);
+        return dropout_op().call(x, residual, p, rng, seed, offset, type);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         refuse_default_stream("dropout");
@@ -275,15 +275,15 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
             dx = dropout_op().call(grads[0], std::nullopt, ctx->saved_data["p"].toDouble(), rng, ctx->saved_data["seed"].toInt(),
                                    ctx->saved_data["offset"].toInt(), (at::ScalarType)ctx->saved_data["type"].toInt());
         }
-        return once({dx, ctx->saved_data["add"].toBool() && ctx->needs_input_grad(1) ? grads[0] : Tensor(), {}, {}, {}, {}});
+        return once({dx, ctx->saved_data["add"].toBool() && ctx->needs_input_grad(1) ? grads[0] : Tensor(), {}, {}, {}, {}, {}});
     }
 };
 
 Tensor dropout_autograd(const Tensor& x, const MaybeTensor& residual, double p, const MaybeTensor& rng, int64_t seed, int64_t offset, MaybeType type) {
     const MaybeTensor input(x);
     refuse_tangents("dropout", {&input, &residual});
-    if (!type && at::GradMode::is_enabled() && (x.requires_grad() || wants_gradient(residual)))
-        return DropoutNode::apply(x, residual, p, rng, seed, offset);
+    if (at::GradMode::is_enabled() && (x.requires_grad() || wants_gradient(residual)))
+        return DropoutNode::apply(x, residual, p, rng, seed, offset, type);
     const at::AutoDispatchBelowADInplaceOrView below;
     return dropout_op().call(x, residual, p, rng, seed, offset, type);
 }
@@ -405,11 +405,12 @@ const auto& norm_backward_op() {
     return op;
 }
 
-// {norm(v), v or nothing} with v = [residual +] dropout(x): one node for the sum, the dropout and the norm
+// {norm(v), v or nothing} with v = [residual +] dropout(x): one node for the sum, the dropout and the norm.  The statistics come out
+// too where a recorded program asks for them, which holds the calls below autograd; they have no derivative.
 struct NormNode : torch::autograd::Function<NormNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight,
                                  const MaybeTensor& bias, int64_t kind, double eps, double p, const MaybeTensor& rng, int64_t seed,
-                                 int64_t offset, bool return_sum) {
+                                 int64_t offset, bool return_sum, bool stats) {
         ctx->set_materialize_grads(false);
         variable_list out;
         {
@@ -417,14 +418,15 @@ struct NormNode : torch::autograd::Function<NormNode> {
             out = norm_op().call(x, residual, weight, bias, kind, eps, p, rng, seed, offset, return_sum, true);
         }
         const Tensor mean = kind == TVAE_NORM_RMS ? Tensor() : out.back(), rstd = out[return_sum ? 2 : 1];
-        out.resize(return_sum ? 2 : 1);
+        if (stats) ctx->mark_non_differentiable(variable_list(out.begin() + (return_sum ? 2 : 1), out.end()));
+        else out.resize(return_sum ? 2 : 1);
         // The backward pass needs v in fp32: it forms it again from x and the residual, or reads the returned sum where that holds
         // v as it is (fp32: 4 bytes an element for the 4 + 2 or 4 + 4 of x and residual).  A 16-bit sum would put its rounding
         // into the weights' gradient.
         const bool kept = return_sum && out[1].scalar_type() == at::kFloat;
         ctx->save_for_backward({kept ? Tensor() : x, kept ? out[1] : tensor_of(residual), tensor_of(weight), mean, rstd, tensor_of(rng)});
         const auto type = [](const MaybeTensor& t) { return t ? (int64_t)t->scalar_type() : (int64_t)-1; };
-        ctx->saved_data["meta"] = std::vector<int64_t>{type(x), type(residual), type(weight), type(bias), kind, seed, offset};
+        ctx->saved_data["meta"] = std::vector<int64_t>{type(x), type(residual), type(weight), type(bias), kind, seed, offset, return_sum};
         ctx->saved_data["p"] = p;
         return out;
     }
@@ -440,7 +442,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
         size_t edge = 0;
         std::array<bool, 4> need;
         for (int i = 0; i < 4; ++i) need[i] = meta[i] >= 0 && ctx->needs_input_grad(edge++);
-        const Tensor dy = grads[0], ds = grads.size() > 1 ? grads[1] : Tensor();
+        const Tensor dy = grads[0], ds = meta[7] ? grads[1] : Tensor();
         Tensor out[4];
         {
             const at::AutoDispatchBelowADInplaceOrView below;
@@ -460,7 +462,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
                 if (shared) out[1] = out[0];
             }
         }
-        return once({out[0], out[1], out[2], out[3], {}, {}, {}, {}, {}, {}, {}});
+        return once({out[0], out[1], out[2], out[3], {}, {}, {}, {}, {}, {}, {}, {}});
     }
 };
 
@@ -468,10 +470,25 @@ std::vector<Tensor> norm_autograd(const Tensor& x, const MaybeTensor& residual, 
                                   double eps, double p, const MaybeTensor& rng, int64_t seed, int64_t offset, bool return_sum, bool stats) {
     const MaybeTensor input(x);
     refuse_tangents("norm", {&input, &residual, &weight, &bias});
-    if (!stats && at::GradMode::is_enabled() && (x.requires_grad() || wants_gradient(residual) || wants_gradient(weight) || wants_gradient(bias)))
-        return NormNode::apply(x, residual, weight, bias, kind, eps, p, rng, seed, offset, return_sum);
+    if (at::GradMode::is_enabled() && (x.requires_grad() || wants_gradient(residual) || wants_gradient(weight) || wants_gradient(bias)))
+        return NormNode::apply(x, residual, weight, bias, kind, eps, p, rng, seed, offset, return_sum, stats);
     const at::AutoDispatchBelowADInplaceOrView below;
     return norm_op().call(x, residual, weight, bias, kind, eps, p, rng, seed, offset, return_sum, stats);
+}
+
+// a recorded backward pass: not to be differentiated again
+std::vector<Tensor> norm_backward_autograd(const Tensor& dy, const MaybeTensor& dsum, const MaybeTensor& x, const MaybeTensor& residual,
+                                           const MaybeTensor& weight, const MaybeTensor& mean, const Tensor& rstd, int64_t kind, double p,
+                                           const MaybeTensor& rng, int64_t seed, int64_t offset, at::ScalarType w_type, std::array<bool, 4> need) {
+    const MaybeTensor first(dy);
+    refuse_tangents("norm_backward", {&first, &dsum, &x, &residual, &weight});
+    std::vector<Tensor> out;
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        out = norm_backward_op().call(dy, dsum, x, residual, weight, mean, rstd, kind, p, rng, seed, offset, w_type, need);
+    }
+    const bool wanted = dy.requires_grad() || wants_gradient(dsum) || wants_gradient(x) || wants_gradient(residual) || wants_gradient(weight);
+    return wanted ? once(std::move(out)) : out;
 }
 
 pybind11::object norm(const char* what, int64_t kind, const Tensor& x, const MaybeTensor& residual, const MaybeTensor& weight,
@@ -509,6 +526,7 @@ TORCH_LIBRARY_IMPL(tvae, Meta, m) {
 TORCH_LIBRARY_IMPL(tvae, Autograd, m) {
     m.impl("dropout", &dropout_autograd);
     m.impl("norm", &norm_autograd);
+    m.impl("norm_backward", &norm_backward_autograd);
 }
 
 PYBIND11_MODULE(_host, m) {
