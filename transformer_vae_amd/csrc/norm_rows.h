@@ -768,7 +768,9 @@ constexpr int NORM_CUS = 256;
 struct RowPlan { int tpr, v; };
 // The shape with the least room that holds the row: idle threads cost what their loads would have brought.  The last list: where x and
 // the residual are of 16 bits (bf16 with dropout and residual, 60000 x 1280: forward 85 us with 64 x 3, 124 with 128 x 2, backward 156
-// and 193); three packs of fp32 do not fit the registers of a fused backward pass.
+// and 193); three packs of fp32 do not fit the registers of a fused backward pass.  They are there for the widths that were measured
+// (768, 1280, 5120).  Not measured: three packs of 16, 128 and 512 threads (bf16, 16384 x 3000: forward 45.5 us with 256 x 2, its bytes
+// alone 32), and three of fp32 without a fused backward pass (60000 x 768 and x 1280 take 2 to 9 % more than their bytes as they are).
 #define NORM_SHAPES(X) X(8, 1) X(16, 1) X(32, 1) X(32, 2) X(64, 2) X(128, 2) X(256, 2) X(512, 2) X(512, 4)
 #define NORM_TINY_SHAPES(X) X(8, 1)
 #define NORM_NARROW_SHAPES(X) X(32, 3) X(64, 3) X(256, 3)

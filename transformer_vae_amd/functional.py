@@ -622,7 +622,8 @@ def _slerp(t1, t2, ratio):
 
 
 # Norms and dropout of the sub-layers around the bottleneck (csrc/norms.hip, csrc/dropout.hip).  Their autograd nodes and the
-# checks of their arguments are C++ (csrc/host.cpp); shapes and values raise ValueError, types TypeError.
+# checks of their arguments are C++ (csrc/host.cpp), registered as torch.ops.tvae; shapes and values raise ValueError, types
+# TypeError, second and forward-mode derivatives RuntimeError and NotImplementedError.
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """Layer norm over the last axis of ``x`` (float32, bfloat16 or float16), differentiable once.  ``weight`` and ``bias`` are
