@@ -91,3 +91,18 @@ def test_double_latents_with_a_dropout_rate(key, L):
     # of their rounding and a rounding a step, within 64 of fp32's in the 2-norm
     assert (out.detach() - want.detach().double()).norm() <= 64 * u_of(F32) * out.detach().norm()
     assert dec.eval()(z).dtype == F64
+
+
+def test_norm_parameters_of_two_types_with_a_dropout_rate():
+    """The default decoder takes them without a rate, and so it does with one."""
+    cfg = t5_cfg(24)
+    cfg.funnel = SimpleNamespace(d_model=64, layer_norm_eps=1e-9)
+    torch.manual_seed(4)
+    dec = amd.VAE_DECODER_MODELS[""](cfg, dropout_rate=0.25).to(dev(), BF16)
+    dec.norm.bias.data = torch.randn(64, device=dev())
+    z = torch.randn(4, 3, 24, device=dev()).to(BF16).requires_grad_(True)
+    assert dec.eval()(z).dtype == BF16
+    out = dec.train()(z)
+    grads = torch.autograd.grad(out.float().square().sum(), [z, *dec.parameters()])
+    assert out.dtype == BF16 and all(torch.isfinite(g).all() for g in grads)
+    assert [g.dtype for g in grads] == [t.dtype for t in (z, *dec.parameters())]

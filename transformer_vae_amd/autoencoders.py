@@ -105,7 +105,9 @@ class LatentDecoderFunnelNorm(LatentDecoderNTokens):
         if p > 0.0:                # LayerNorm(dropout(linear)), as the Funnel's own sub-layers order them
             out = self._decode(latent)
             r = _single(out)
-            g, c = (t if t.dtype in (r.dtype, torch.float32) else t.float() for t in (self.norm.weight, self.norm.bias))
+            g, c = self.norm.weight, self.norm.bias
+            if not g.dtype == c.dtype == r.dtype:
+                g, c = g.float(), c.float()
             return F.dropout_add_layer_norm(r, None, g, c, self.norm.eps, p).to(out.dtype)
         return F.latent_decode(latent, w, b, self.norm.weight, self.norm.bias, self.norm.eps)
 
